@@ -37,8 +37,10 @@ extern "C" {
  * network -- sdeh_zrec_floats, sdeh_simulate_fwd_train3, sdeh_ctrl_backward_fused_z; plan option SDEH_BWD_ZREC.
  * v7 (round 6): BASELINE configs[4]'s target -- the NICE flow (distr/nice.py) as a row-parallel log-density + score evaluation
  * (SdehNice, sdeh_nice_work_floats, sdeh_nice_eval), a target whose score is SUPPLIED per step (SDEH_DENS_EXTERNAL) and the wide
- * kernels run in segments of the time grid around it (sdeh_simulate_fwd_steps). */
-#define SDEH_ABI_VERSION 7
+ * kernels run in segments of the time grid around it (sdeh_simulate_fwd_steps).
+ * v8: training a policy on trajectories drawn before the update -- sdeh_step_log_ratio[_backward], sdeh_policy_loss, sdeh_preference_loss,
+ * sdeh_preference_grad -- and an optimizer step of its own: sdeh_adamw_step, sdeh_adamw_moments. */
+#define SDEH_ABI_VERSION 8
 #define SDEH_MAX_HIDDEN 8 /* max entries of any nn.ModuleList of hidden layers */
 
 typedef enum {
@@ -533,6 +535,124 @@ int32_t sdeh_guard_restore(const uint64_t* table, int32_t n_tensors, const uint8
 /* importance weights exp(-rnd - m) (losses/oc.py:101-103) with a caller-provided global maximum m (device scalar). */
 int32_t sdeh_importance_weights(const float* rnd, int64_t batch, const float* log_weight_max, float* weights,
                                 void* stream);
+
+/*
+ * ABI v8: losses over trajectories that were drawn before the update, and the update itself.
+ *
+ * Tensors of these entry points may be fp32, bf16 or fp16 (SdehDtype); sums, softmax-like statistics and optimizer moments are held in 32
+ * or 64 bits whatever the inputs' type, every output is rounded once.  Nothing allocates or synchronises; scratch is the caller's and is
+ * needed until the launches have run.  Captured into a graph, a replay reads the same pointers again.
+ */
+typedef enum { SDEH_F32 = 0, SDEH_BF16 = 1, SDEH_F16 = 2 } SdehDtype;
+
+/* Log-ratio of the Gaussian Euler-Maruyama steps of two controls of one SDE (the Girsanov weight of a single step; the quantity that
+ * losses/oc.py:204-219 accumulates over a trajectory), for paths driven by `increments` dW under the control `behaviour` v:
+ *   log_ratio[t, b] = sum_d (u - v) dW  -  1/2 dt[t] sum_d (u - v)^2
+ * control, behaviour (NULL = 0), increments: [n_steps, batch, dim] contiguous, one dtype;  dt [n_steps] fp32;  log_ratio [n_steps, batch] fp32.
+ * _backward: grad_control = grad[t, b] (dW - dt (u - v)), grad [n_steps, batch] fp32, grad_control like control. */
+int32_t sdeh_step_log_ratio(const void* control, const void* behaviour, const void* increments, const float* dt, int64_t n_steps,
+                            int64_t batch, int32_t dim, int32_t dtype, float* log_ratio, void* stream);
+int32_t sdeh_step_log_ratio_backward(const void* control, const void* behaviour, const void* increments, const float* dt, const float* grad,
+                                     int64_t n_steps, int64_t batch, int32_t dim, int32_t dtype, void* grad_control, void* stream);
+
+/* Clipped policy loss with a KL term over [rows, steps] log-probabilities.  Per valid entry, with delta = log_prob - old_log_prob and
+ * r = exp(delta):
+ *   surrogate = -min(A r, A clip(r, 1 - clip_low, 1 + clip_high)), for A < 0 and dual_clip > 1 at most -A dual_clip
+ *   kl        = k | k^2 / 2 | exp(-k) - 1 + k          with k = log_prob - ref_log_prob (SdehKlEstimator)
+ *   loss      = sum w (surrogate + kl_coef kl),  w = 1 / N | 1 / (rows with a valid entry x valid entries of the row) | 1 (SdehReduction)
+ * Entries whose mask is 0 are not read into any result, whatever they hold; with no valid entry the loss and its gradient are 0.
+ * Which side of a clipping border r lies on is decided on delta in 64 bits. */
+typedef enum { SDEH_KL_1 = 1, SDEH_KL_2 = 2, SDEH_KL_3 = 3 } SdehKlEstimator;
+typedef enum { SDEH_REDUCE_STEPS = 0, SDEH_REDUCE_ROWS = 1, SDEH_REDUCE_SUM = 2 } SdehReduction;
+typedef struct {
+  const void* data;        /* NULL = absent */
+  int64_t row_stride;      /* in elements; 0 broadcasts */
+  int64_t step_stride;
+} SdehPlane;
+typedef struct {
+  SdehPlane log_prob, old_log_prob /* NULL = 0 */, ref_log_prob /* NULL = no KL term */, advantage;
+  SdehPlane mask;          /* bytes, 0 = padding; NULL = every entry is valid */
+  int64_t rows, steps;
+  int32_t dtype;           /* of log_prob, old_log_prob, ref_log_prob and grad */
+  int32_t advantage_dtype;
+  int32_t kl, reduction;
+  double clip_low, clip_high, dual_clip /* 0 = none */, kl_coef;
+} SdehPolicyLoss;
+int64_t sdeh_policy_loss_scratch_floats(int64_t rows);
+/* out (nullable) [5] fp32 = loss, sum w surrogate, sum w kl, clipped share of the valid entries, their number.
+ * grad (nullable) [rows, steps] contiguous, dtype: d loss / d log_prob x grad_factor x *grad_scale (fp32 on the device, NULL = 1).
+ * reuse_counts != 0: scratch still holds what an earlier call with the same mask and reduction left there (a loss's backward pass). */
+int32_t sdeh_policy_loss(const SdehPolicyLoss* p, float* scratch, int32_t reuse_counts, const float* grad_scale, float grad_factor, float* out,
+                         void* grad, void* stream);
+
+/* Preference loss of `pairs` paired rows: with s = sum over the row's valid entries of (log_prob - ref_log_prob) (their mean when average != 0;
+ * 0 for a row without any) and h = beta (s_chosen - s_rejected)
+ *   logistic  -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h)   |   hinge  max(0, 1 - h)   |
+ *   square    (s_chosen - s_rejected - 1 / (2 beta))^2                       averaged over the pairs. */
+typedef enum { SDEH_PREF_LOGISTIC = 0, SDEH_PREF_HINGE = 1, SDEH_PREF_SQUARE = 2 } SdehPreferenceKind;
+typedef struct {
+  SdehPlane log_prob, ref_log_prob /* NULL = 0 */, mask /* bytes; NULL = every entry */;
+  int64_t steps;
+} SdehPreferenceSide;
+typedef struct {
+  SdehPreferenceSide chosen, rejected;
+  int64_t pairs;
+  int32_t dtype;
+  int32_t kind, average;
+  double beta, label_smoothing;
+} SdehPreferenceLoss;
+int64_t sdeh_preference_loss_scratch_floats(const SdehPreferenceLoss* p);
+/* out [2 + 4 pairs] fp32: loss, share of pairs with h > 0, then per pair beta s_chosen, beta s_rejected, d loss / d (each valid chosen entry),
+ * d loss / d (each valid rejected entry).  grad_chosen / grad_rejected (nullable, both or none): [pairs, steps] contiguous, dtype, x grad_factor. */
+int32_t sdeh_preference_loss(const SdehPreferenceLoss* p, float* scratch, float grad_factor, float* out, void* grad_chosen, void* grad_rejected,
+                             void* stream);
+/* the gradients alone, from `out` of sdeh_preference_loss, x grad_factor x *grad_scale (nullable) */
+int32_t sdeh_preference_grad(const SdehPreferenceLoss* p, const float* out, const float* grad_scale, float grad_factor, void* grad_chosen,
+                             void* grad_rejected, void* stream);
+
+/* One AdamW step over n tensors (decoupled weight decay; with weight_decay 0: Adam), gradients clipped by their global norm when max_norm > 0:
+ *   c = min(1, max_norm / (norm + 1e-6));   g' = c g;   m = beta1 m + (1 - beta1) g';   v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps),   t = ++(*step)
+ * state_bits 32: exp_avg, exp_avg_sq fp32 [numel].  state_bits 8: one byte per entry, and one byte per block of SDEH_MOMENT_BLOCK entries, the
+ * block's largest exponent `top` (biased, as fp32 stores it).  Code c > 0 stands for 2^(top - 127 - depth + c / 8) (1 + (c % 8) / 8) (integer
+ * division), 0 for 0, with depth = 15 and the sign in bit 7 for exp_avg, depth = 31 and eight bits for exp_avg_sq.  A moment is rounded to its
+ * three mantissa bits stochastically, with 16 bits that are a function of (seed, t, place): rounding to the nearest would leave a second moment
+ * where it is whenever (1 - beta2) moves it by less than half a code.  place = SDEH_MOMENT_BLOCK first_block + index.
+ * ok (nullable): one byte on the device; 0 leaves parameters, moments and step counters as they are. */
+#define SDEH_MOMENT_BLOCK 256
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  uint8_t* exp_avg_top;    /* state_bits 8: [ceil(numel / SDEH_MOMENT_BLOCK)] */
+  uint8_t* exp_avg_sq_top;
+  float* step;             /* one fp32 counter */
+  int64_t numel;
+  int64_t first_block;     /* place of the tensor among the optimizer's blocks */
+} SdehAdamwTensor;
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* lr_dev;     /* nullable: the learning rate on the device, instead of lr */
+  int32_t n_tensors;
+  int32_t dtype;           /* of params */
+  int32_t grad_dtype;
+  int32_t state_bits;
+} SdehAdamwGroup;
+typedef struct {
+  double max_norm;         /* 0 = no clipping; the norm is that of the gradients of all groups */
+  const uint8_t* ok;
+  float* norm;             /* nullable [1]: the gradients' norm before clipping (max_norm > 0 only) */
+  uint32_t seed;
+  int32_t n_groups;
+} SdehAdamw;
+/* tensors: those of the first group, then those of the second, ..  They must not overlap, and no counter may serve two of them.
+ * scratch: 16-byte aligned, sdeh_adamw_scratch_floats(all tensors). */
+int64_t sdeh_adamw_scratch_floats(int32_t n_tensors);
+int32_t sdeh_adamw_step(const SdehAdamw* p, const SdehAdamwGroup* groups, const SdehAdamwTensor* tensors, float* scratch, void* stream);
+/* The fp32 values that 8-bit moments stand for: `blocks` whole blocks of codes -> exp_avg, exp_avg_sq [blocks * SDEH_MOMENT_BLOCK] */
+int32_t sdeh_adamw_moments(const uint8_t* exp_avg, const uint8_t* exp_avg_top, const uint8_t* exp_avg_sq, const uint8_t* exp_avg_sq_top,
+                           int64_t blocks, float* exp_avg_out, float* exp_avg_sq_out, void* stream);
 
 /*
  * Plain Euler-Maruyama integration with output-time interpolation.  Replaces EulerIntegrator.integrate

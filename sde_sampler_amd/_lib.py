@@ -8,9 +8,10 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
-SDEH_ABI_VERSION = 7
+SDEH_ABI_VERSION = 8
 SDEH_NICE_MAX_COUPLING = 8
 SDEH_MAX_HIDDEN = 8
 SDEH_REDUCE_SCRATCH = 8192
@@ -27,6 +28,17 @@ FLAG_TERMINAL_TARGET, FLAG_TERMINAL_SECOND, FLAG_REFERENCE_CTRL = 16, 32, 64
 FLAG_INFERENCE_SDE, FLAG_INFERENCE_CTRL = 128, 256
 FLAG_DETACH_SCORE, FLAG_TARGET_SCORE_CONST = 512, 1024
 INT_LANGEVIN, INT_CONTROLLED = 0, 1
+F32, BF16, F16 = 0, 1, 2
+KL_ESTIMATORS = {"k1": 1, "k2": 2, "k3": 3}
+REDUCTIONS = {"steps": 0, "rows": 1, "sum": 2}
+PREFERENCE_KINDS = {"logistic": 0, "hinge": 1, "square": 2}
+MOMENT_BLOCK = 256
+# structs of the loss / optimizer entry points, packed in one go (native alignment, as in include/sdeh.h)
+POLICY_LOSS = struct.Struct("@" + "Pqq" * 5 + "qq4i4d")
+PREFERENCE_LOSS = struct.Struct("@" + ("Pqq" * 3 + "q") * 2 + "q3i2d")
+ADAMW_GROUP = struct.Struct("@5dP4i")
+ADAMW = struct.Struct("@dPPIi")
+ADAMW_TENSOR_WORDS = 9  # SdehAdamwTensor: seven pointers, two int64
 DENS_FLAG_SHARED_SCALE = 1
 DENS_FLAG_MM_OK = 2  # the mixture's logits may be evaluated in product form (engine._mixture_mm_ok)
 
@@ -201,6 +213,16 @@ PROTOTYPES = {
     "sdeh_partial_sums": (C.c_int32, [fp, C.c_int64, C.c_int64, C.c_int64, fp, fp, C.c_void_p]),
     "sdeh_weight_grad": (C.c_int32, [fp, C.c_int32, fp, C.c_int32, C.c_int64, C.c_int32, C.c_int64, fp, fp, C.c_void_p]),
     "sdeh_reduce_estimators": (C.c_int32, [fp, C.c_int64, C.c_float, fp, fp, C.c_void_p]),
+    "sdeh_step_log_ratio": (C.c_int32, [fp, fp, fp, fp, C.c_int64, C.c_int64, C.c_int32, C.c_int32, fp, C.c_void_p]),
+    "sdeh_step_log_ratio_backward": (C.c_int32, [fp, fp, fp, fp, fp, C.c_int64, C.c_int64, C.c_int32, C.c_int32, fp, C.c_void_p]),
+    "sdeh_policy_loss_scratch_floats": (C.c_int64, [C.c_int64]),
+    "sdeh_policy_loss": (C.c_int32, [C.c_char_p, fp, C.c_int32, fp, C.c_float, fp, fp, C.c_void_p]),
+    "sdeh_preference_loss_scratch_floats": (C.c_int64, [C.c_char_p]),
+    "sdeh_preference_loss": (C.c_int32, [C.c_char_p, fp, C.c_float, fp, fp, fp, C.c_void_p]),
+    "sdeh_preference_grad": (C.c_int32, [C.c_char_p, fp, fp, C.c_float, fp, fp, C.c_void_p]),
+    "sdeh_adamw_scratch_floats": (C.c_int64, [C.c_int32]),
+    "sdeh_adamw_step": (C.c_int32, [C.c_char_p, C.c_char_p, fp, fp, C.c_void_p]),
+    "sdeh_adamw_moments": (C.c_int32, [fp, fp, fp, fp, C.c_int64, fp, fp, C.c_void_p]),
     "sdeh_importance_weights": (C.c_int32, [fp, C.c_int64, fp, fp, C.c_void_p]),
     "sdeh_debug_philox": (C.c_int32, [C.c_uint64, C.c_uint64, C.c_int64, C.c_int32, C.c_int32, C.c_int64, fp, C.c_void_p]),
     "sdeh_debug_normals": (C.c_int32, [C.c_uint64, C.c_uint64, C.c_int64, C.c_int32, C.c_int32, C.c_int64, fp, C.c_void_p]),
@@ -242,6 +264,29 @@ def load():
         raise SdehLibraryError(f"ABI mismatch: library {lib.sdeh_abi_version()} != binding {SDEH_ABI_VERSION}")
     _LIB = lib
     return lib
+
+
+def dtype_code(dtype) -> int | None:
+    """SdehDtype of a torch dtype, None where the kernels have none."""
+    import torch
+
+    return {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}.get(dtype)
+
+
+def call(name: str, device, *args):
+    """Calls a stream-ordered entry point on torch's current stream of `device` (its last argument), whichever device is current."""
+    import torch
+
+    fn = getattr(load(), name)
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, stream)
+    if status != 0:
+        check(status)
 
 
 def check(status: int):

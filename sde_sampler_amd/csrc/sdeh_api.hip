@@ -19,6 +19,19 @@ int launch_loss_moment(const float* rnd, long long n, float max_rnd, int lv, lon
                        hipStream_t stream);
 int launch_guard_restore(const unsigned long long* table, int n_tensors, const unsigned char* ok, long long* n_skipped, hipStream_t stream);
 int launch_guard_check(float* g, long long n, const float* value, float max_loss, unsigned char* ok, hipStream_t stream);
+int launch_step_log_ratio(const void* u, const void* v, const void* dw, const float* dt, const float* g, long long n_steps, long long batch, int dim,
+                          int dtype, void* out, hipStream_t stream);                                                        // sdeh_policy.hip
+long long policy_scratch_floats(long long rows);
+int launch_policy_loss(const SdehPolicyLoss& p, float* scratch, int reuse_counts, const float* grad_scale, float grad_factor, float* out, void* grad,
+                       hipStream_t stream);
+long long preference_scratch_floats(const SdehPreferenceLoss& p);
+int launch_preference_loss(const SdehPreferenceLoss& p, float* scratch, float grad_factor, float* out, void* grad_c, void* grad_r, hipStream_t stream);
+int launch_preference_grad(const SdehPreferenceLoss& p, const float* out, const float* grad_scale, float grad_factor, void* grad_c, void* grad_r,
+                           hipStream_t stream);
+long long adamw_scratch_floats(int n_tensors);                                                                              // sdeh_adamw.hip
+int launch_adamw_step(const SdehAdamw& p, const SdehAdamwGroup* groups, const SdehAdamwTensor* tensors, float* scratch, hipStream_t stream);
+int launch_adamw_moments(const uint8_t* m, const uint8_t* m_top, const uint8_t* v, const uint8_t* v_top, long long blocks, float* om, float* ov,
+                         hipStream_t stream);
 int launch_sink_init(float* u, float* v, float* log_a, float* log_b, const float* w_x, const float* w_y, long long n,
                      long long m, float eps, int* flags, hipStream_t st);
 int launch_sink_finalize(const float* pm, const float* ps, int splits, long long np, const float* log_w, float eps, float* pot,
@@ -1967,6 +1980,122 @@ int32_t sdeh_importance_weights(const float* rnd, int64_t batch, const float* lo
     return fail(SDEH_ERR_INVALID, "importance_weights: bad argument");
   const int rc = launch_weights(rnd, batch, log_weight_max, weights, (hipStream_t)stream);
   return rc == SDEH_OK ? SDEH_OK : fail(rc, "importance_weights: launch failed");
+}
+
+// ---- ABI v8: losses over trajectories drawn before the update, the optimizer step -------------------------------------------------------
+static bool dtype_ok(int32_t t) { return t == SDEH_F32 || t == SDEH_BF16 || t == SDEH_F16; }
+
+static int32_t step_log_ratio(const char* who, const void* control, const void* behaviour, const void* increments, const float* dt, const float* grad,
+                              int64_t n_steps, int64_t batch, int32_t dim, int32_t dtype, void* out, bool back, void* stream) {
+  if (n_steps < 0 || batch < 0 || dim < 1 || !dtype_ok(dtype)) return fail(SDEH_ERR_INVALID, "%s: bad size or type", who);
+  if (n_steps == 0 || batch == 0) return SDEH_OK;
+  if (control == nullptr || increments == nullptr || dt == nullptr || out == nullptr || (back && grad == nullptr))
+    return fail(SDEH_ERR_INVALID, "%s: null pointer", who);
+  if (n_steps > INT64_MAX / 16 / batch / dim) return fail(SDEH_ERR_INVALID, "%s: too many elements", who);
+  const int rc = launch_step_log_ratio(control, behaviour, increments, dt, grad, n_steps, batch, dim, dtype, out, (hipStream_t)stream);
+  return rc == SDEH_OK ? SDEH_OK : fail(rc, rc == SDEH_ERR_UNSUPPORTED ? "%s: more rows than one launch holds" : "%s: launch failed", who);
+}
+
+int32_t sdeh_step_log_ratio(const void* control, const void* behaviour, const void* increments, const float* dt, int64_t n_steps, int64_t batch,
+                            int32_t dim, int32_t dtype, float* log_ratio, void* stream) {
+  return step_log_ratio("step_log_ratio", control, behaviour, increments, dt, nullptr, n_steps, batch, dim, dtype, log_ratio, false, stream);
+}
+
+int32_t sdeh_step_log_ratio_backward(const void* control, const void* behaviour, const void* increments, const float* dt, const float* grad,
+                                     int64_t n_steps, int64_t batch, int32_t dim, int32_t dtype, void* grad_control, void* stream) {
+  return step_log_ratio("step_log_ratio_backward", control, behaviour, increments, dt, grad, n_steps, batch, dim, dtype, grad_control, true, stream);
+}
+
+int64_t sdeh_policy_loss_scratch_floats(int64_t rows) { return rows < 0 ? 0 : policy_scratch_floats(rows); }
+
+int32_t sdeh_policy_loss(const SdehPolicyLoss* p, float* scratch, int32_t reuse_counts, const float* grad_scale, float grad_factor, float* out,
+                         void* grad, void* stream) {
+  if (p == nullptr || scratch == nullptr || (out == nullptr && grad == nullptr)) return fail(SDEH_ERR_INVALID, "policy_loss: null pointer");
+  if (p->rows < 0 || p->steps < 0 || p->steps > INT32_MAX || (p->rows > 0 && p->steps > INT64_MAX / 16 / p->rows))
+    return fail(SDEH_ERR_INVALID, "policy_loss: bad size");
+  if (p->rows > 0 && p->steps > 0 && (p->log_prob.data == nullptr || p->advantage.data == nullptr))
+    return fail(SDEH_ERR_INVALID, "policy_loss: log_prob and advantage are needed");
+  if (!dtype_ok(p->dtype) || !dtype_ok(p->advantage_dtype)) return fail(SDEH_ERR_INVALID, "policy_loss: unknown type");
+  if (p->kl < SDEH_KL_1 || p->kl > SDEH_KL_3 || p->reduction < SDEH_REDUCE_STEPS || p->reduction > SDEH_REDUCE_SUM)
+    return fail(SDEH_ERR_INVALID, "policy_loss: unknown KL estimator or reduction");
+  if (!(p->clip_low >= 0.0) || !(p->clip_high >= 0.0) || !(p->dual_clip == 0.0 || p->dual_clip > 1.0))
+    return fail(SDEH_ERR_INVALID, "policy_loss: clip_low and clip_high are >= 0, dual_clip is 0 or > 1");
+  const int rc = launch_policy_loss(*p, scratch, reuse_counts, grad_scale, grad_factor, out, grad, (hipStream_t)stream);
+  return rc == SDEH_OK ? SDEH_OK : fail(rc, "policy_loss: launch failed");
+}
+
+static int32_t preference_ok(const SdehPreferenceLoss* p) {
+  if (p == nullptr) return fail(SDEH_ERR_INVALID, "preference_loss: null pointer");
+  if (p->pairs < 1 || p->chosen.steps < 0 || p->rejected.steps < 0 || p->chosen.steps > INT64_MAX / 32 / p->pairs ||
+      p->rejected.steps > INT64_MAX / 32 / p->pairs)
+    return fail(SDEH_ERR_INVALID, "preference_loss: bad size");
+  if (!dtype_ok(p->dtype) || p->kind < SDEH_PREF_LOGISTIC || p->kind > SDEH_PREF_SQUARE)
+    return fail(SDEH_ERR_INVALID, "preference_loss: unknown type or kind");
+  if ((p->chosen.log_prob.data == nullptr && p->chosen.steps > 0) || (p->rejected.log_prob.data == nullptr && p->rejected.steps > 0))
+    return fail(SDEH_ERR_INVALID, "preference_loss: both sides' log_prob are needed");
+  if (!(p->beta > 0.0) || !(p->label_smoothing >= 0.0 && p->label_smoothing < 0.5))
+    return fail(SDEH_ERR_INVALID, "preference_loss: beta > 0 and 0 <= label_smoothing < 0.5");
+  return SDEH_OK;
+}
+
+int64_t sdeh_preference_loss_scratch_floats(const SdehPreferenceLoss* p) { return p == nullptr || p->pairs < 1 ? 0 : preference_scratch_floats(*p); }
+
+int32_t sdeh_preference_loss(const SdehPreferenceLoss* p, float* scratch, float grad_factor, float* out, void* grad_chosen, void* grad_rejected,
+                             void* stream) {
+  if (const int32_t bad = preference_ok(p); bad != SDEH_OK) return bad;
+  if (scratch == nullptr || out == nullptr || (grad_chosen == nullptr) != (grad_rejected == nullptr))
+    return fail(SDEH_ERR_INVALID, "preference_loss: null pointer");
+  const int rc = launch_preference_loss(*p, scratch, grad_factor, out, grad_chosen, grad_rejected, (hipStream_t)stream);
+  return rc == SDEH_OK ? SDEH_OK : fail(rc, "preference_loss: launch failed");
+}
+
+int32_t sdeh_preference_grad(const SdehPreferenceLoss* p, const float* out, const float* grad_scale, float grad_factor, void* grad_chosen,
+                             void* grad_rejected, void* stream) {
+  if (const int32_t bad = preference_ok(p); bad != SDEH_OK) return bad;
+  if (out == nullptr || grad_chosen == nullptr || grad_rejected == nullptr) return fail(SDEH_ERR_INVALID, "preference_grad: null pointer");
+  const int rc = launch_preference_grad(*p, out, grad_scale, grad_factor, grad_chosen, grad_rejected, (hipStream_t)stream);
+  return rc == SDEH_OK ? SDEH_OK : fail(rc, "preference_grad: launch failed");
+}
+
+int64_t sdeh_adamw_scratch_floats(int32_t n_tensors) { return n_tensors < 0 ? 0 : adamw_scratch_floats(n_tensors); }
+
+int32_t sdeh_adamw_step(const SdehAdamw* p, const SdehAdamwGroup* groups, const SdehAdamwTensor* tensors, float* scratch, void* stream) {
+  if (p == nullptr || groups == nullptr || scratch == nullptr || p->n_groups < 0 || !(p->max_norm >= 0.0))
+    return fail(SDEH_ERR_INVALID, "adamw_step: bad argument");
+  if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return fail(SDEH_ERR_INVALID, "adamw_step: scratch is not aligned to 16 bytes");
+  int64_t at = 0;
+  for (int32_t k = 0; k < p->n_groups; ++k) {
+    const SdehAdamwGroup& g = groups[k];
+    if (!dtype_ok(g.dtype) || !dtype_ok(g.grad_dtype) || (g.state_bits != 8 && g.state_bits != 32))
+      return fail(SDEH_ERR_INVALID, "adamw_step: unknown type, or moments in neither 8 nor 32 bits");
+    if (!(g.beta1 >= 0.0 && g.beta1 < 1.0) || !(g.beta2 >= 0.0 && g.beta2 < 1.0) || !(g.eps >= 0.0) || !(g.lr >= 0.0) || !(g.weight_decay >= 0.0))
+      return fail(SDEH_ERR_INVALID, "adamw_step: lr, eps and weight_decay are >= 0, betas in [0, 1)");
+    if (g.n_tensors < 0 || (g.n_tensors > 0 && tensors == nullptr)) return fail(SDEH_ERR_INVALID, "adamw_step: bad argument");
+    for (const int64_t end = at + g.n_tensors; at < end; ++at) {
+      const SdehAdamwTensor& t = tensors[at];
+      if (t.numel < 0 || t.first_block < 0 || t.step == nullptr ||
+          (t.numel > 0 && (t.param == nullptr || t.grad == nullptr || t.exp_avg == nullptr || t.exp_avg_sq == nullptr ||
+                           (g.state_bits == 8 && (t.exp_avg_top == nullptr || t.exp_avg_sq_top == nullptr)))))
+        return fail(SDEH_ERR_INVALID, "adamw_step: tensor %d: null pointer or bad size", (int)at);
+    }
+  }
+  if (at == 0) return SDEH_OK;
+  const int rc = launch_adamw_step(*p, groups, tensors, scratch, (hipStream_t)stream);
+  return rc == SDEH_OK ? SDEH_OK : fail(rc, rc == SDEH_ERR_UNSUPPORTED ? "adamw_step: more tensors or entries than one call takes" : "adamw_step: launch failed");
+}
+
+int32_t sdeh_adamw_moments(const uint8_t* exp_avg, const uint8_t* exp_avg_top, const uint8_t* exp_avg_sq, const uint8_t* exp_avg_sq_top,
+                           int64_t blocks, float* exp_avg_out, float* exp_avg_sq_out, void* stream) {
+  if (blocks < 0) return fail(SDEH_ERR_INVALID, "adamw_moments: bad size");
+  if (blocks == 0) return SDEH_OK;
+  if (exp_avg == nullptr || exp_avg_top == nullptr || exp_avg_sq == nullptr || exp_avg_sq_top == nullptr || exp_avg_out == nullptr ||
+      exp_avg_sq_out == nullptr)
+    return fail(SDEH_ERR_INVALID, "adamw_moments: null pointer");
+  if (((reinterpret_cast<uintptr_t>(exp_avg) | reinterpret_cast<uintptr_t>(exp_avg_sq)) & 3) != 0 ||
+      ((reinterpret_cast<uintptr_t>(exp_avg_out) | reinterpret_cast<uintptr_t>(exp_avg_sq_out)) & 15) != 0)
+    return fail(SDEH_ERR_INVALID, "adamw_moments: codes are aligned to 4 bytes, values to 16");
+  const int rc = launch_adamw_moments(exp_avg, exp_avg_top, exp_avg_sq, exp_avg_sq_top, blocks, exp_avg_out, exp_avg_sq_out, (hipStream_t)stream);
+  return rc == SDEH_OK ? SDEH_OK : fail(rc, "adamw_moments: launch failed");
 }
 
 }  // extern "C"

@@ -1,0 +1,62 @@
+// Elements of fp32 / bf16 / fp16 tensors in registers, and sums over a workgroup: shared by the kernels that stream caller tensors
+// (sdeh_policy.hip, sdeh_adamw.hip).
+#pragma once
+#include "sdeh_common.hpp"
+
+namespace sdeh {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// V neighbours, loaded and stored as one access (V * sizeof(T) = 16 bytes, or less)
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+  T v[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_pack(const T* __restrict__ p, float (&x)[V]) {
+  const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = static_cast<float>(k.v[i]);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&x)[V]) {
+  Pack<T, V> k;
+#pragma unroll
+  for (int i = 0; i < V; ++i) k.v[i] = static_cast<T>(x[i]);  // (to nearest even: the one rounding of an output)
+  *reinterpret_cast<Pack<T, V>*>(p) = k;
+}
+
+// one element of a tensor whose type is known at run time
+__device__ __forceinline__ float load_as(const void* p, int dtype, long long i) {
+  if (dtype == SDEH_F32) return static_cast<const float*>(p)[i];
+  if (dtype == SDEH_BF16) return static_cast<float>(static_cast<const bf16_t*>(p)[i]);
+  return static_cast<float>(static_cast<const f16_t*>(p)[i]);
+}
+
+template <typename A>
+__device__ __forceinline__ A wave_sum(A x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+  return x;
+}
+
+// the sum over a workgroup of NT threads, in every thread and in an order that does not change from call to call
+template <int NT, typename A>
+__device__ __forceinline__ A block_sum(A x) {
+  __shared__ A part[NT / 64];
+  x = wave_sum(x);
+  __syncthreads();  // (an earlier sum's readers are done)
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+  __syncthreads();
+  A s = part[0];
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) s += part[w];
+  return s;
+}
+
+inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+}  // namespace sdeh

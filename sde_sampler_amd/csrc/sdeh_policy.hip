@@ -1,0 +1,997 @@
+// Losses over trajectories drawn before the update: the step log-ratio of two controls, the clipped policy loss with a KL term and the
+// preference loss, each with its gradient (include/sdeh.h, ABI v8).  All of them are streams over [rows, steps] or [steps, batch, dim] tensors
+// with a handful of operations per element: bounded by memory, and by their launches below about 1e5 entries.
+#include "sdeh_elem.hpp"
+
+namespace sdeh {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// -------------------------------------------------------------------------------------------------------------------------------------------
+// step log-ratio: l = sum_d e dW - dt/2 e^2, e = u - v;   gradient g (dW - dt e)
+//
+// A row is one trajectory at one step, dim coordinates: 1 .. a few hundred, seldom a multiple of what a lane loads at once.  A workgroup
+// therefore takes `rows` whole rows -- one contiguous stretch, loaded 16 bytes a lane whatever dim is --, puts the elements' terms into LDS and
+// sums the rows from there with G lanes a row.  dt differs from row to row only where a stretch passes the end of a step; it is staged per row.
+// -------------------------------------------------------------------------------------------------------------------------------------------
+constexpr int kStretch = 4096;      // elements of a stretch, at most (16 KB of terms)
+constexpr int kStretchRows = 1024;  // rows of a stretch, at most
+constexpr int kStagedDim = 512;     // rows longer than this are summed by a workgroup each, without LDS
+
+struct RatioArgs {
+  const void* u;
+  const void* v;
+  const void* dw;
+  const float* dt;
+  const float* g;
+  void* out;
+  long long rows_total, batch;
+  int dim, rows, group;  // rows per stretch, lanes per row
+};
+
+template <typename T, int V, bool BACK>
+__global__ __launch_bounds__(kThreads) void ratio_kernel(RatioArgs a) {
+  __shared__ float term[BACK ? 1 : kStretch + kStretch / 32];
+  __shared__ float row_dt[kStretchRows];
+  __shared__ float row_g[BACK ? kStretchRows : 1];
+  const long long r0 = (long long)blockIdx.x * a.rows;
+  const int nr = (int)(a.rows_total - r0 < a.rows ? a.rows_total - r0 : a.rows);
+  const int d = a.dim, n = nr * d;
+  const long long t0 = r0 / a.batch;  // (uniform over the workgroup)
+  const long long b0 = r0 - t0 * a.batch;
+  for (int r = threadIdx.x; r < nr; r += kThreads) {
+    const long long b = b0 + r, t = b < a.batch ? t0 : t0 + b / a.batch;
+    row_dt[r] = a.dt[t];
+    if (BACK) row_g[r] = a.g[r0 + r];
+  }
+  __syncthreads();
+  const T* u = static_cast<const T*>(a.u) + r0 * d;
+  const T* v = a.v == nullptr ? nullptr : static_cast<const T*>(a.v) + r0 * d;
+  const T* dw = static_cast<const T*>(a.dw) + r0 * d;
+  T* out = static_cast<T*>(a.out) + r0 * d;
+  for (int i = threadIdx.x * V; i < n; i += kThreads * V) {
+    float xu[V], xv[V], xw[V];
+    const int live = n - i < V ? n - i : V;
+    if (live == V) {
+      load_pack<T, V>(u + i, xu);
+      load_pack<T, V>(dw + i, xw);
+      if (v != nullptr) load_pack<T, V>(v + i, xv);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        xu[k] = k < live ? (float)u[i + k] : 0.0f;
+        xw[k] = k < live ? (float)dw[i + k] : 0.0f;
+        if (v != nullptr) xv[k] = k < live ? (float)v[i + k] : 0.0f;
+      }
+    }
+    int r = (int)((unsigned)i / (unsigned)d), c = i - r * d;
+    float dt = row_dt[r], g = BACK ? row_g[r] : 0.0f;
+    float y[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float e = xu[k] - (v != nullptr ? xv[k] : 0.0f);
+      if (BACK) {
+        y[k] = g * (xw[k] - dt * e);
+      } else {
+        term[i + k + ((i + k) >> 5)] = e * (xw[k] - 0.5f * dt * e);  // (one word of padding in 32: rows of 32, 64, .. words spread over the banks)
+      }
+      if (++c == d && k + 1 < live) {
+        c = 0;
+        ++r;
+        dt = row_dt[r];
+        if (BACK) g = row_g[r];
+      }
+    }
+    if (BACK) {
+      if (live == V) {
+        store_pack<T, V>(out + i, y);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (k < live) out[i + k] = static_cast<T>(y[k]);
+      }
+    }
+  }
+  if (!BACK) {
+    __syncthreads();
+    const int G = a.group, lane = threadIdx.x & (G - 1);
+    for (int r = threadIdx.x / G; r < nr; r += kThreads / G) {
+      float s = 0.0f;
+      for (int j = lane; j < d; j += G) {
+        const int w = r * d + j;
+        s += term[w + (w >> 5)];
+      }
+      for (int o = G >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+      if (lane == 0) static_cast<float*>(a.out)[r0 + r] = s;
+    }
+  }
+}
+
+// rows longer than kStagedDim: a workgroup sums one
+template <typename T>
+__global__ __launch_bounds__(kThreads) void ratio_long_kernel(RatioArgs a) {
+  const long long row = blockIdx.x, base = row * a.dim;
+  const T* u = static_cast<const T*>(a.u) + base;
+  const T* v = a.v == nullptr ? nullptr : static_cast<const T*>(a.v) + base;
+  const T* dw = static_cast<const T*>(a.dw) + base;
+  const float half_dt = 0.5f * a.dt[row / a.batch];
+  float s = 0.0f;
+  for (int i = threadIdx.x; i < a.dim; i += kThreads) {
+    const float e = (float)u[i] - (v != nullptr ? (float)v[i] : 0.0f);
+    s += e * ((float)dw[i] - half_dt * e);
+  }
+  s = block_sum<kThreads>(s);
+  if (threadIdx.x == 0) static_cast<float*>(a.out)[row] = s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void ratio_long_back_kernel(RatioArgs a) {
+  const long long row = blockIdx.x, base = row * a.dim;
+  const T* u = static_cast<const T*>(a.u) + base;
+  const T* v = a.v == nullptr ? nullptr : static_cast<const T*>(a.v) + base;
+  const T* dw = static_cast<const T*>(a.dw) + base;
+  T* out = static_cast<T*>(a.out) + base;
+  const float dt = a.dt[row / a.batch], g = a.g[row];
+  for (int i = threadIdx.x; i < a.dim; i += kThreads) {
+    const float e = (float)u[i] - (v != nullptr ? (float)v[i] : 0.0f);
+    out[i] = static_cast<T>(g * ((float)dw[i] - dt * e));
+  }
+}
+
+template <typename T, bool BACK>
+int launch_ratio_t(RatioArgs a, hipStream_t stream) {
+  if (a.dim > kStagedDim) {
+    if (a.rows_total > 0x7FFFFFFFll) return SDEH_ERR_UNSUPPORTED;
+    if (BACK)
+      hipLaunchKernelGGL(ratio_long_back_kernel<T>, dim3((unsigned)a.rows_total), dim3(kThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL(ratio_long_kernel<T>, dim3((unsigned)a.rows_total), dim3(kThreads), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? SDEH_OK : SDEH_ERR_HIP;
+  }
+  // whole rows, a multiple of eight of them: every stretch then starts at a multiple of 16 bytes
+  int rows = kStretch / a.dim / 8 * 8;
+  a.rows = rows > kStretchRows ? kStretchRows : rows;
+  a.group = 1;
+  while (a.group < 64 && a.group * 2 * a.rows <= kThreads && a.group * 2 <= a.dim) a.group *= 2;
+  const long long blocks = (a.rows_total + a.rows - 1) / a.rows;
+  if (blocks > 0x7FFFFFFFll) return SDEH_ERR_UNSUPPORTED;
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool wide = aligned_to(a.u, 16) && aligned_to(a.dw, 16) && (a.v == nullptr || aligned_to(a.v, 16)) && (!BACK || aligned_to(a.out, 16));
+  if (wide)
+    hipLaunchKernelGGL((ratio_kernel<T, V, BACK>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((ratio_kernel<T, 1, BACK>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+  return hipGetLastError() == hipSuccess ? SDEH_OK : SDEH_ERR_HIP;
+}
+
+}  // namespace
+
+int launch_step_log_ratio(const void* u, const void* v, const void* dw, const float* dt, const float* g, long long n_steps, long long batch,
+                          int dim, int dtype, void* out, hipStream_t stream) {
+  RatioArgs a{u, v, dw, dt, g, out, n_steps * batch, batch, dim, 0, 0};
+  if (g != nullptr)
+    return dtype == SDEH_F32 ? launch_ratio_t<float, true>(a, stream)
+                             : dtype == SDEH_BF16 ? launch_ratio_t<bf16_t, true>(a, stream) : launch_ratio_t<f16_t, true>(a, stream);
+  return dtype == SDEH_F32 ? launch_ratio_t<float, false>(a, stream)
+                           : dtype == SDEH_BF16 ? launch_ratio_t<bf16_t, false>(a, stream) : launch_ratio_t<f16_t, false>(a, stream);
+}
+
+namespace {
+
+// -------------------------------------------------------------------------------------------------------------------------------------------
+// clipped policy loss
+//
+// One pass reads every input once, forms the entry's loss and slope and writes the gradient; what it needs beforehand is the weight of an
+// entry, i.e. how many entries are valid -- a pass over the mask's bytes alone (1 of 14 to 21 bytes an entry), which leaves partial counts that
+// every workgroup of the main pass adds up again.  No atomics, no last-workgroup ticket: results do not depend on the order of workgroups and
+// nothing has to be cleared between calls.
+// -------------------------------------------------------------------------------------------------------------------------------------------
+constexpr int kCountBlocks = 512, kPolicyBlocks = 2048, kSmallThreads = 1024;
+
+struct PolicyArgs {
+  SdehPolicyLoss p;
+  long long n;          // rows * steps
+  long long d_row, d_col;  // (rows, steps) that one iteration of the grid moves an entry by
+  double log_hi, log_lo, log_dual;
+  float hi, lo, dual, kl_coef;
+  const float* grad_scale;
+  float grad_factor;
+  void* grad;
+  float* out;
+  int* row_count;       // [rows]              scratch
+  long long* part_n;    // [kCountBlocks]
+  double* part;         // [kPolicyBlocks][4]
+  int n_count, n_part;  // workgroups of the two passes
+  bool flat_advantage;  // fp32, laid out like the other planes
+};
+
+__device__ __forceinline__ bool needs_counts(const PolicyArgs& a) { return a.p.mask.data != nullptr && a.p.reduction != SDEH_REDUCE_SUM; }
+
+// non-zero bytes of m[0 .. n), the share of thread `me` of `team`
+__device__ __forceinline__ int count_span(const uint8_t* m, long long n, long long stride, long long me, long long team) {
+  int c = 0;
+  if (stride != 1) {
+    for (long long i = me; i < n; i += team) c += m[i * stride] != 0;
+    return c;
+  }
+  const long long to_border = (16 - (reinterpret_cast<uintptr_t>(m) & 15)) & 15, head = to_border < n ? to_border : n;
+  const long long packs = (n - head) / 16;
+  for (long long i = me; i < head; i += team) c += m[i] != 0;
+#pragma unroll 4
+  for (long long i = me; i < packs; i += team) {
+    const Pack<uint8_t, 16> k = *reinterpret_cast<const Pack<uint8_t, 16>*>(m + head + 16 * i);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) c += k.v[j] != 0;
+  }
+  for (long long i = head + 16 * packs + me; i < n; i += team) c += m[i] != 0;
+  return c;
+}
+
+// What the weights divide by, this workgroup's share: valid entries (SDEH_REDUCE_STEPS) or rows that have one (SDEH_REDUCE_ROWS; the row
+// counts are kept).  A wave counts a row, of more than kLongRow entries the workgroup; a dense mask of SDEH_REDUCE_STEPS is one span.
+constexpr long long kLongRow = 4096;
+
+template <int NT>
+__device__ __forceinline__ void count_pass(const PolicyArgs& a) {
+  const uint8_t* m = static_cast<const uint8_t*>(a.p.mask.data);
+  const long long T = a.p.steps;
+  long long mine = 0;
+  if (a.p.reduction == SDEH_REDUCE_STEPS && a.p.mask.step_stride == 1 && a.p.mask.row_stride == T) {
+    mine = count_span(m, a.n, 1, (long long)blockIdx.x * NT + threadIdx.x, (long long)gridDim.x * NT);
+  } else if (T > kLongRow) {
+    for (long long row = blockIdx.x; row < a.p.rows; row += gridDim.x) {
+      const int c = block_sum<NT>(count_span(m + row * a.p.mask.row_stride, T, a.p.mask.step_stride, threadIdx.x, NT));
+      if (threadIdx.x == 0) {
+        a.row_count[row] = c;
+        mine += a.p.reduction == SDEH_REDUCE_ROWS ? c != 0 : c;
+      }
+    }
+  } else {
+    const int lane = threadIdx.x & 63;
+    for (long long row = (long long)blockIdx.x * (NT / 64) + (threadIdx.x >> 6); row < a.p.rows; row += (long long)gridDim.x * (NT / 64)) {
+      const int c = wave_sum(count_span(m + row * a.p.mask.row_stride, T, a.p.mask.step_stride, lane, 64));
+      if (lane == 0) {
+        a.row_count[row] = c;
+        mine += a.p.reduction == SDEH_REDUCE_ROWS ? c != 0 : c;
+      }
+    }
+  }
+  mine = block_sum<NT>(mine);
+  if (threadIdx.x == 0) a.part_n[blockIdx.x] = mine;
+}
+
+// The weight that all entries have in common.
+template <int NT>
+__device__ __forceinline__ double common_weight(const PolicyArgs& a, int n_count) {
+  if (a.p.reduction == SDEH_REDUCE_SUM) return 1.0;
+  long long n = a.p.reduction == SDEH_REDUCE_ROWS ? a.p.rows : a.n;
+  if (a.p.mask.data != nullptr) {
+    long long s = 0;
+    for (int i = threadIdx.x; i < n_count; i += NT) s += a.part_n[i];
+    n = block_sum<NT>(s);
+  }
+  return 1.0 / (double)(n > 0 ? n : 1);
+}
+
+// exp(-k) - 1 + k and its slope 1 - exp(-k).  Below |k| = 1/2 by its series (the difference would lose the digits that exp(-k) and 1 - k share):
+// k^2 (1/2! - k/3! + ... + k^8/10!), the first term left out is below 1e-10 of the sum.
+__device__ __forceinline__ float kl3(float k, float& slope) {
+  const float e = expf(-k);
+  const float far = (e - 1.0f) + k;
+  float s = 2.7557319e-7f;
+  s = fmaf(-k, s, 2.7557319e-6f);
+  s = fmaf(-k, s, 2.4801587e-5f);
+  s = fmaf(-k, s, 1.9841270e-4f);
+  s = fmaf(-k, s, 1.3888889e-3f);
+  s = fmaf(-k, s, 8.3333333e-3f);
+  s = fmaf(-k, s, 4.1666667e-2f);
+  s = fmaf(-k, s, 1.6666667e-1f);
+  s = fmaf(-k, s, 0.5f);
+  const float near = k * k * s;
+  const bool small = fabsf(k) < 0.5f;
+  slope = small ? k - near : 1.0f - e;
+  return small ? near : far;
+}
+
+struct PolicySums {
+  double policy, kl;
+  long long clipped, valid;
+};
+
+// All entries, V neighbours a thread.  V > 1: every plane is contiguous and aligned; V = 1: any strides.
+template <typename T, int V, int NT>
+__device__ __forceinline__ PolicySums policy_pass(const PolicyArgs& a, double w_common) {
+  PolicySums sums{0.0, 0.0, 0, 0};
+  const SdehPolicyLoss& p = a.p;
+  const T* lp = static_cast<const T*>(p.log_prob.data);
+  const T* old = static_cast<const T*>(p.old_log_prob.data);
+  const T* ref = static_cast<const T*>(p.ref_log_prob.data);
+  const uint8_t* mask = static_cast<const uint8_t*>(p.mask.data);
+  T* grad = static_cast<T*>(a.grad);
+  const bool row_adv = V > 1 && p.advantage.step_stride == 0;
+  const bool flat_adv = V > 1 && a.flat_advantage;
+  const bool row_weight = p.reduction == SDEH_REDUCE_ROWS;
+  const float w_all = (float)w_common, w_dense = row_weight ? (float)(w_common / (double)p.steps) : w_all;
+  const float factor = a.grad_factor * (a.grad_scale != nullptr ? *a.grad_scale : 1.0f);
+  const long long stride = (long long)gridDim.x * NT * V;
+  long long i = ((long long)blockIdx.x * NT + threadIdx.x) * V;
+  if (i >= a.n) return sums;
+  long long row = i / p.steps, col = i - row * p.steps;
+  for (; i < a.n; i += stride) {
+    const int live = a.n - i < V ? (int)(a.n - i) : V;
+    bool ok[V];
+    int any = 0;
+    if (mask == nullptr) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) ok[k] = k < live;
+      any = 1;
+    } else if (V > 1 && live == V) {
+      const Pack<uint8_t, V> m = *reinterpret_cast<const Pack<uint8_t, V>*>(mask + i);
+#pragma unroll
+      for (int k = 0; k < V; ++k) any |= ok[k] = m.v[k] != 0;
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        ok[k] = k < live && mask[V > 1 ? i + k : row * p.mask.row_stride + col * p.mask.step_stride] != 0;
+        any |= ok[k];
+      }
+    }
+    float g[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) g[k] = 0.0f;
+    if (any) {  // (a stretch of padding is neither read nor computed)
+      float x[V], o[V], q[V], adv[V];
+      if (V > 1 && live == V) {
+        load_pack<T, V>(lp + i, x);
+        if (old != nullptr) load_pack<T, V>(old + i, o);
+        if (ref != nullptr) load_pack<T, V>(ref + i, q);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const bool in = k < live;
+          x[k] = in ? (float)lp[V > 1 ? i + k : row * p.log_prob.row_stride + col * p.log_prob.step_stride] : 0.0f;
+          if (old != nullptr) o[k] = in ? (float)old[V > 1 ? i + k : row * p.old_log_prob.row_stride + col * p.old_log_prob.step_stride] : 0.0f;
+          if (ref != nullptr) q[k] = in ? (float)ref[V > 1 ? i + k : row * p.ref_log_prob.row_stride + col * p.ref_log_prob.step_stride] : 0.0f;
+        }
+      }
+      if (flat_adv && live == V) {
+        if constexpr (V > 4) {
+          float half[4];
+#pragma unroll
+          for (int j = 0; j < V; j += 4) {
+            load_pack<float, 4>(static_cast<const float*>(p.advantage.data) + i + j, half);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) adv[j + k] = half[k];
+          }
+        } else {
+          load_pack<float, V>(static_cast<const float*>(p.advantage.data) + i, adv);
+        }
+      }
+      float w[V];
+      {
+        long long r = row, c = col;
+        float a_row = 0.0f, w_row = w_dense;
+        bool fresh = true;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          if (fresh && k < live) {
+            if (row_adv) a_row = load_as(p.advantage.data, p.advantage_dtype, r * p.advantage.row_stride);
+            if (row_weight && mask != nullptr) w_row = w_all / (float)a.row_count[r];  // (only entries of rows that have one are weighed)
+          }
+          adv[k] = row_adv                    ? a_row
+                   : flat_adv && live == V ? adv[k]
+                   : k < live ? load_as(p.advantage.data, p.advantage_dtype, r * p.advantage.row_stride + c * p.advantage.step_stride) : 0.0f;
+          w[k] = w_row;
+          fresh = ++c == p.steps;
+          if (fresh) {
+            c = 0;
+            ++r;
+          }
+        }
+      }
+      float s_policy = 0.0f, s_kl = 0.0f;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const double delta = old != nullptr ? (double)x[k] - (double)o[k] : (double)x[k];
+        const bool over = delta > a.log_hi, under = delta < a.log_lo;
+        const float A = adv[k];
+        bool clipped = (A > 0.0f && over) || (A < 0.0f && under);
+        float bound = over ? a.hi : a.lo;
+        if (A < 0.0f && delta > a.log_dual) {
+          clipped = true;
+          bound = a.dual;
+        }
+        const float used = clipped ? bound : expf((float)delta);
+        const float surrogate = A == 0.0f ? 0.0f : -A * used;
+        float slope = clipped ? 0.0f : surrogate;
+        float kl = 0.0f;
+        if (ref != nullptr) {
+          const float d = (float)((double)x[k] - (double)q[k]);
+          float kl_slope;
+          if (p.kl == SDEH_KL_3) {
+            kl = kl3(d, kl_slope);
+          } else if (p.kl == SDEH_KL_2) {
+            kl = 0.5f * d * d;
+            kl_slope = d;
+          } else {
+            kl = d;
+            kl_slope = 1.0f;
+          }
+          slope = fmaf(a.kl_coef, kl_slope, slope);
+        }
+        s_policy += ok[k] ? (row_weight ? surrogate * w[k] : surrogate) : 0.0f;
+        s_kl += ok[k] ? (row_weight ? kl * w[k] : kl) : 0.0f;
+        sums.clipped += ok[k] && clipped;
+        sums.valid += ok[k];
+        g[k] = ok[k] ? slope * w[k] * factor : 0.0f;
+      }
+      sums.policy += (double)s_policy;
+      sums.kl += (double)s_kl;
+    }
+    if (grad != nullptr) {
+      if (V > 1 && live == V) {
+        store_pack<T, V>(grad + i, g);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (k < live) grad[i + k] = static_cast<T>(g[k]);
+      }
+    }
+    row += a.d_row;
+    col += a.d_col;
+    if (col >= p.steps) {
+      col -= p.steps;
+      ++row;
+    }
+  }
+  return sums;
+}
+
+// out = loss, policy, kl, clipped share, valid entries; the sums of SDEH_REDUCE_STEPS still want their common weight
+__device__ __forceinline__ void policy_result(const PolicyArgs& a, double policy, double kl, double clipped, double valid) {
+  const double n = valid > 0.0 ? valid : 1.0;
+  if (a.p.reduction == SDEH_REDUCE_STEPS) {
+    policy /= n;
+    kl /= n;
+  }
+  a.out[0] = (float)(policy + a.p.kl_coef * kl);
+  a.out[1] = (float)policy;
+  a.out[2] = (float)kl;
+  a.out[3] = (float)(clipped / n);
+  a.out[4] = (float)valid;
+}
+
+template <int NT>
+__global__ __launch_bounds__(NT) void policy_count_kernel(PolicyArgs a) {
+  count_pass<NT>(a);
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void policy_kernel(PolicyArgs a) {
+  const double w = common_weight<kThreads>(a, a.n_count);
+  const PolicySums s = policy_pass<T, V, kThreads>(a, w);
+  if (a.out == nullptr) return;
+  const double policy = block_sum<kThreads>(s.policy), kl = block_sum<kThreads>(s.kl);
+  const long long clipped = block_sum<kThreads>(s.clipped), valid = block_sum<kThreads>(s.valid);
+  if (threadIdx.x == 0) {
+    double* o = a.part + 4 * blockIdx.x;
+    o[0] = policy;
+    o[1] = kl;
+    o[2] = (double)clipped;
+    o[3] = (double)valid;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void policy_final_kernel(PolicyArgs a) {
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int i = threadIdx.x; i < a.n_part; i += kThreads)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] += a.part[4 * i + k];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s[k] = block_sum<kThreads>(s[k]);
+  if (threadIdx.x == 0) policy_result(a, s[0], s[1], s[2], s[3]);
+}
+
+// few entries: counting, the pass and the result by one workgroup in one launch
+template <typename T, int V>
+__global__ __launch_bounds__(kSmallThreads) void policy_small_kernel(PolicyArgs a) {
+  if (needs_counts(a)) {
+    count_pass<kSmallThreads>(a);
+    __threadfence_block();
+    __syncthreads();
+  }
+  const double w = common_weight<kSmallThreads>(a, 1);
+  const PolicySums s = policy_pass<T, V, kSmallThreads>(a, w);
+  if (a.out == nullptr) return;
+  const double policy = block_sum<kSmallThreads>(s.policy), kl = block_sum<kSmallThreads>(s.kl);
+  const long long clipped = block_sum<kSmallThreads>(s.clipped), valid = block_sum<kSmallThreads>(s.valid);
+  if (threadIdx.x == 0) policy_result(a, policy, kl, (double)clipped, (double)valid);
+}
+
+constexpr long long kPolicySmall = 8192;  // entries that one workgroup takes
+
+bool dense(const SdehPlane& q, long long steps, size_t bytes) {
+  return q.data == nullptr || (q.step_stride == 1 && q.row_stride == steps && aligned_to(q.data, bytes));
+}
+
+template <typename T>
+int launch_policy_t(PolicyArgs a, bool reuse_counts, hipStream_t stream) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const SdehPolicyLoss& p = a.p;
+  const bool adv_ok = p.advantage.step_stride == 0 || p.advantage.step_stride == 1;
+  const bool wide = dense(p.log_prob, p.steps, 16) && dense(p.old_log_prob, p.steps, 16) && dense(p.ref_log_prob, p.steps, 16) &&
+                    dense(p.mask, p.steps, V) && adv_ok && aligned_to(a.grad, 16);
+  a.flat_advantage = wide && p.advantage_dtype == SDEH_F32 && dense(p.advantage, p.steps, 16);
+  const int v = wide ? V : 1;
+  const bool small = a.n <= kPolicySmall;
+  const int nt = small ? kSmallThreads : kThreads;
+  long long blocks = (a.n + (long long)nt * v - 1) / ((long long)nt * v);
+  blocks = small ? 1 : blocks > kPolicyBlocks ? kPolicyBlocks : blocks;
+  const long long stride = blocks * nt * v;
+  a.d_row = p.steps > 0 ? stride / p.steps : 0;
+  a.d_col = p.steps > 0 ? stride % p.steps : 0;
+  a.n_part = (int)blocks;
+  if (small) {
+    if (wide)
+      hipLaunchKernelGGL((policy_small_kernel<T, V>), dim3(1), dim3(kSmallThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL((policy_small_kernel<T, 1>), dim3(1), dim3(kSmallThreads), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? SDEH_OK : SDEH_ERR_HIP;
+  }
+  const bool span = p.reduction == SDEH_REDUCE_STEPS && p.mask.step_stride == 1 && p.mask.row_stride == p.steps, long_rows = p.steps > kLongRow;
+  const long long count_blocks = span ? (a.n + 16 * kThreads - 1) / (16 * kThreads) : long_rows ? p.rows : (p.rows + kThreads / 64 - 1) / (kThreads / 64);
+  a.n_count = (int)(count_blocks > kCountBlocks ? kCountBlocks : count_blocks);
+  if (p.mask.data != nullptr && p.reduction != SDEH_REDUCE_SUM && !reuse_counts) {
+    if (long_rows && !span)
+      hipLaunchKernelGGL(policy_count_kernel<kSmallThreads>, dim3(a.n_count), dim3(kSmallThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL(policy_count_kernel<kThreads>, dim3(a.n_count), dim3(kThreads), 0, stream, a);
+  }
+  if (wide)
+    hipLaunchKernelGGL((policy_kernel<T, V>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((policy_kernel<T, 1>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+  if (a.out != nullptr) hipLaunchKernelGGL(policy_final_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+  return hipGetLastError() == hipSuccess ? SDEH_OK : SDEH_ERR_HIP;
+}
+
+}  // namespace
+
+// scratch: partial sums, partial counts, row counts
+long long policy_scratch_floats(long long rows) { return kPolicyBlocks * 8ll + kCountBlocks * 2ll + (rows + 1) / 2 * 2; }
+
+int launch_policy_loss(const SdehPolicyLoss& p, float* scratch, int reuse_counts, const float* grad_scale, float grad_factor, float* out,
+                       void* grad, hipStream_t stream) {
+  PolicyArgs a{};
+  a.p = p;
+  a.n = p.rows * p.steps;
+  a.log_hi = log1p(p.clip_high);
+  a.log_lo = p.clip_low < 1.0 ? log1p(-p.clip_low) : -HUGE_VAL;
+  a.log_dual = p.dual_clip > 0.0 ? log(p.dual_clip) : HUGE_VAL;
+  a.hi = (float)(1.0 + p.clip_high);
+  a.lo = (float)(1.0 - p.clip_low);
+  a.dual = (float)p.dual_clip;
+  a.kl_coef = (float)p.kl_coef;
+  a.grad_scale = grad_scale;
+  a.grad_factor = grad_factor;
+  a.grad = grad;
+  a.out = out;
+  a.part = reinterpret_cast<double*>(scratch);
+  a.part_n = reinterpret_cast<long long*>(scratch + kPolicyBlocks * 8ll);
+  a.row_count = reinterpret_cast<int*>(scratch + kPolicyBlocks * 8ll + kCountBlocks * 2ll);
+  return p.dtype == SDEH_F32 ? launch_policy_t<float>(a, reuse_counts != 0, stream)
+                             : p.dtype == SDEH_BF16 ? launch_policy_t<bf16_t>(a, reuse_counts != 0, stream)
+                                                    : launch_policy_t<f16_t>(a, reuse_counts != 0, stream);
+}
+
+namespace {
+
+// -------------------------------------------------------------------------------------------------------------------------------------------
+// preference loss: sums of the rows (split over their length where rows are few and long), the pairs, the gradients
+//
+// A pair's slope is known only when both its rows are summed, so the gradient -- the slope again and again, 0 in the padding -- is a second
+// pass; it reads nothing but the mask.
+// -------------------------------------------------------------------------------------------------------------------------------------------
+constexpr int kPairBlocks = 256;
+
+struct PreferenceArgs {
+  SdehPreferenceLoss p;
+  int splits;               // parts of a row
+  long long chunk;          // entries of a part
+  double* sum;              // [2 pairs][splits]   scratch
+  long long* count;         // [2 pairs][splits]
+  double* part;             // [kPairBlocks][2]
+  int n_pair_blocks;
+  float* out;
+  const float* slopes;      // [2][pairs]
+  const float* grad_scale;
+  float grad_factor;
+  void* grad[2];
+  long long d_row[2], d_col[2];
+};
+
+// Sum and number of the valid entries [lo, hi) of a row, this thread's share: `me` of `team` threads.
+template <typename T, int V>
+__device__ __forceinline__ void row_share(const SdehPreferenceSide& s, long long row, long long lo, long long hi, int me, int team, double& sum,
+                                          long long& count) {
+  const T* x = static_cast<const T*>(s.log_prob.data) + row * s.log_prob.row_stride;
+  const T* q = s.ref_log_prob.data == nullptr ? nullptr : static_cast<const T*>(s.ref_log_prob.data) + row * s.ref_log_prob.row_stride;
+  const uint8_t* m = s.mask.data == nullptr ? nullptr : static_cast<const uint8_t*>(s.mask.data) + row * s.mask.row_stride;
+  const auto one = [&](long long i) {
+    if (m == nullptr || m[i * s.mask.step_stride] != 0) {
+      const double a = (double)(float)x[i * s.log_prob.step_stride];
+      sum += q == nullptr ? a : a - (double)(float)q[i * s.ref_log_prob.step_stride];
+      ++count;
+    }
+  };
+  if (V == 1) {
+    for (long long i = lo + me; i < hi; i += team) one(i);
+    return;
+  }
+  // contiguous planes with one row stride: entries up to the first 16-byte border (the same in every plane), vectors, the rest
+  const long long flat = row * s.log_prob.row_stride;
+  long long head = lo + (V - (flat + lo) % V) % V;
+  if (head > hi) head = hi;
+  const long long body = head + (hi - head) / V * V;
+  for (long long i = lo + me; i < head; i += team) one(i);
+  for (long long i = head + (long long)me * V; i < body; i += (long long)team * V) {
+    bool ok[V];
+    int any = 1;
+    if (m != nullptr) {
+      const Pack<uint8_t, V> k = *reinterpret_cast<const Pack<uint8_t, V>*>(m + i);
+      any = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) any |= ok[j] = k.v[j] != 0;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) ok[j] = true;
+    }
+    if (any) {
+      float a[V], b[V];
+      load_pack<T, V>(x + i, a);
+      if (q != nullptr) load_pack<T, V>(q + i, b);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const double d = q == nullptr ? (double)a[j] : (double)a[j] - (double)b[j];
+        sum += ok[j] ? d : 0.0;
+        count += ok[j];
+      }
+    }
+  }
+  for (long long i = body + me; i < hi; i += team) one(i);
+}
+
+// one workgroup a part of a row
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void preference_sum_kernel(PreferenceArgs a) {
+  const long long line = blockIdx.x / a.splits;
+  const int split = blockIdx.x % a.splits;
+  const bool second = line >= a.p.pairs;
+  const SdehPreferenceSide& s = second ? a.p.rejected : a.p.chosen;
+  const long long lo = split * a.chunk, hi = lo + a.chunk < s.steps ? lo + a.chunk : s.steps;
+  double sum = 0.0;
+  long long count = 0;
+  if (lo < hi) row_share<T, V>(s, second ? line - a.p.pairs : line, lo, hi, threadIdx.x, kThreads, sum, count);
+  sum = block_sum<kThreads>(sum);
+  count = block_sum<kThreads>(count);
+  if (threadIdx.x == 0) {
+    a.sum[blockIdx.x] = sum;
+    a.count[blockIdx.x] = count;
+  }
+}
+
+// short rows: one wave a row
+template <typename T, int V, int NT>
+__device__ __forceinline__ void short_rows(const PreferenceArgs& a, long long first, long long step) {
+  for (long long line = first; line < 2 * a.p.pairs; line += step) {
+    const bool second = line >= a.p.pairs;
+    const SdehPreferenceSide& s = second ? a.p.rejected : a.p.chosen;
+    double sum = 0.0;
+    long long count = 0;
+    row_share<T, V>(s, second ? line - a.p.pairs : line, 0, s.steps, threadIdx.x & 63, 64, sum, count);
+    sum = wave_sum(sum);
+    count = wave_sum(count);
+    if ((threadIdx.x & 63) == 0) {
+      a.sum[line] = sum;
+      a.count[line] = count;
+    }
+  }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void preference_short_kernel(PreferenceArgs a) {
+  short_rows<T, V, kThreads>(a, (long long)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), (long long)gridDim.x * (kThreads / 64));
+}
+
+// loss and slope of one pair from its rows' sums; adds to (loss, correct)
+__device__ __forceinline__ void one_pair(const PreferenceArgs& a, long long i, double sc, long long nc, double sr, long long nr, double& loss,
+                                         double& correct) {
+  const long long P = a.p.pairs;
+  double wc = 1.0, wr = 1.0;
+  if (a.p.average) {
+    wc = 1.0 / (double)(nc > 0 ? nc : 1);
+    wr = 1.0 / (double)(nr > 0 ? nr : 1);
+  }
+  sc *= wc;
+  sr *= wr;
+  const double beta = a.p.beta, gap = sc - sr, h = beta * gap, eps = a.p.label_smoothing;
+  double l, slope;
+  if (a.p.kind == SDEH_PREF_LOGISTIC) {
+    const double e = exp(-fabs(h)), tail = log1p(e);  // -log sigmoid(+-h) = log1p(e^-|h|) + max(-+h, 0)
+    l = (1.0 - eps) * (tail + (h < 0.0 ? -h : 0.0)) + (eps > 0.0 ? eps * (tail + (h > 0.0 ? h : 0.0)) : 0.0);
+    const double away = h >= 0.0 ? e / (1.0 + e) : 1.0 / (1.0 + e);  // sigmoid(-h)
+    slope = beta * (eps - away);
+  } else if (a.p.kind == SDEH_PREF_HINGE) {
+    l = h < 1.0 ? 1.0 - h : 0.0;
+    slope = h < 1.0 ? -beta : 0.0;
+    if (h != h) l = slope = h;
+  } else {
+    const double r = gap - 0.5 / beta;
+    l = r * r;
+    slope = 2.0 * r;
+  }
+  slope /= (double)P;
+  float* o = a.out + 2;
+  o[i] = (float)(beta * sc);
+  o[P + i] = (float)(beta * sr);
+  o[2 * P + i] = (float)(slope * wc);
+  o[3 * P + i] = (float)(-slope * wr);
+  loss += l;
+  correct += h > 0.0 ? 1.0 : 0.0;
+}
+
+// splits == 1: a thread a pair, else a wave
+template <int NT>
+__device__ __forceinline__ void pairs_pass(const PreferenceArgs& a, double& loss, double& correct) {
+  const long long P = a.p.pairs;
+  const int S = a.splits;
+  if (S == 1) {
+    for (long long i = (long long)blockIdx.x * NT + threadIdx.x; i < P; i += (long long)gridDim.x * NT)
+      one_pair(a, i, a.sum[i], a.count[i], a.sum[P + i], a.count[P + i], loss, correct);
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  for (long long i = (long long)blockIdx.x * (NT / 64) + (threadIdx.x >> 6); i < P; i += (long long)gridDim.x * (NT / 64)) {
+    double s[2] = {0.0, 0.0};
+    long long n[2] = {0, 0};
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      for (int k = lane; k < S; k += 64) {
+        s[side] += a.sum[(side * P + i) * S + k];
+        n[side] += a.count[(side * P + i) * S + k];
+      }
+      s[side] = wave_sum(s[side]);
+      n[side] = wave_sum(n[side]);
+    }
+    if (lane == 0) one_pair(a, i, s[0], n[0], s[1], n[1], loss, correct);
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void preference_pair_kernel(PreferenceArgs a) {
+  double loss = 0.0, correct = 0.0;
+  pairs_pass<kThreads>(a, loss, correct);
+  loss = block_sum<kThreads>(loss);
+  correct = block_sum<kThreads>(correct);
+  if (threadIdx.x == 0) {
+    const double P = (double)a.p.pairs;
+    if (gridDim.x == 1) {
+      a.out[0] = (float)(loss / P);
+      a.out[1] = (float)(correct / P);
+    } else {
+      a.part[2 * blockIdx.x] = loss;
+      a.part[2 * blockIdx.x + 1] = correct;
+    }
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void preference_final_kernel(PreferenceArgs a) {
+  double loss = 0.0, correct = 0.0;
+  for (int i = threadIdx.x; i < a.n_pair_blocks; i += kThreads) {
+    loss += a.part[2 * i];
+    correct += a.part[2 * i + 1];
+  }
+  loss = block_sum<kThreads>(loss);
+  correct = block_sum<kThreads>(correct);
+  if (threadIdx.x == 0) {
+    a.out[0] = (float)(loss / (double)a.p.pairs);
+    a.out[1] = (float)(correct / (double)a.p.pairs);
+  }
+}
+
+// gradients of one side: the pair's slope on valid entries
+template <typename T, int V, int NT>
+__device__ __forceinline__ void spread_pass(const PreferenceArgs& a, int side, const float* slopes) {
+  const SdehPreferenceSide& s = side ? a.p.rejected : a.p.chosen;
+  const uint8_t* m = static_cast<const uint8_t*>(s.mask.data);
+  T* grad = static_cast<T*>(a.grad[side]);
+  const float factor = a.grad_factor * (a.grad_scale != nullptr ? *a.grad_scale : 1.0f);
+  const long long n = a.p.pairs * s.steps, stride = (long long)gridDim.x * NT * V;
+  long long i = ((long long)blockIdx.x * NT + threadIdx.x) * V;
+  if (i >= n) return;
+  long long row = i / s.steps, col = i - row * s.steps;
+  for (; i < n; i += stride) {
+    const int live = n - i < V ? (int)(n - i) : V;
+    long long r = row, c = col;
+    float g[V], slope = slopes[r] * factor;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const bool ok = k < live && (m == nullptr || V > 1 || m[r * s.mask.row_stride + c * s.mask.step_stride] != 0);
+      g[k] = ok ? slope : 0.0f;
+      if (++c == s.steps && k + 1 < live) {
+        c = 0;
+        ++r;
+        slope = slopes[r] * factor;
+      }
+    }
+    if (V > 1 && live == V) {
+      if (m != nullptr) {
+        const Pack<uint8_t, V> k8 = *reinterpret_cast<const Pack<uint8_t, V>*>(m + i);
+#pragma unroll
+        for (int k = 0; k < V; ++k) g[k] = k8.v[k] != 0 ? g[k] : 0.0f;
+      }
+      store_pack<T, V>(grad + i, g);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (k < live) grad[i + k] = static_cast<T>(m == nullptr || V == 1 || m[i + k] != 0 ? g[k] : 0.0f);
+    }
+    row += a.d_row[side];
+    col += a.d_col[side];
+    if (col >= s.steps) {
+      col -= s.steps;
+      ++row;
+    }
+  }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void preference_grad_kernel(PreferenceArgs a) {
+  const int side = blockIdx.y;
+  spread_pass<T, V, kThreads>(a, side, a.slopes + side * a.p.pairs);
+}
+
+// few and short rows: everything by one workgroup
+template <typename T, int V>
+__global__ __launch_bounds__(kSmallThreads) void preference_small_kernel(PreferenceArgs a) {
+  short_rows<T, V, kSmallThreads>(a, threadIdx.x >> 6, kSmallThreads / 64);
+  __threadfence_block();
+  __syncthreads();
+  double loss = 0.0, correct = 0.0;
+  pairs_pass<kSmallThreads>(a, loss, correct);
+  __threadfence_block();
+  loss = block_sum<kSmallThreads>(loss);
+  correct = block_sum<kSmallThreads>(correct);
+  if (threadIdx.x == 0) {
+    a.out[0] = (float)(loss / (double)a.p.pairs);
+    a.out[1] = (float)(correct / (double)a.p.pairs);
+  }
+  if (a.grad[0] != nullptr) {
+    spread_pass<T, V, kSmallThreads>(a, 0, a.out + 2 + 2 * a.p.pairs);
+    spread_pass<T, V, kSmallThreads>(a, 1, a.out + 2 + 3 * a.p.pairs);
+  }
+}
+
+constexpr long long kPreferenceSmall = 8192;  // entries of both sides that one workgroup takes
+constexpr long long kShortRow = 1024;         // rows that a wave sums
+constexpr int kMaxSplits = 64;
+
+// parts of a row: a workgroup a part, and 1024 workgroups where rows are few
+int preference_splits(const SdehPreferenceLoss& p) {
+  const long long longest = p.chosen.steps > p.rejected.steps ? p.chosen.steps : p.rejected.steps;
+  if (longest <= kShortRow) return 1;
+  long long s = (1024 + 2 * p.pairs - 1) / (2 * p.pairs), most = (longest + 4095) / 4096;
+  s = s > most ? most : s;
+  return (int)(s > kMaxSplits ? kMaxSplits : s < 1 ? 1 : s);
+}
+
+bool dense_side(const SdehPreferenceSide& s, int v) {
+  return dense(s.log_prob, s.steps, 16) && dense(s.ref_log_prob, s.steps, 16) && dense(s.mask, s.steps, v);
+}
+
+void grad_strides(PreferenceArgs& a, long long blocks, int nt, int v) {
+  const long long steps[2] = {a.p.chosen.steps, a.p.rejected.steps};
+  for (int k = 0; k < 2; ++k) {
+    a.d_row[k] = steps[k] > 0 ? blocks * nt * v / steps[k] : 0;
+    a.d_col[k] = steps[k] > 0 ? blocks * nt * v % steps[k] : 0;
+  }
+}
+
+template <typename T>
+int launch_spread_t(PreferenceArgs a, hipStream_t stream) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const SdehPreferenceLoss& p = a.p;
+  const bool wide = dense(p.chosen.mask, p.chosen.steps, V) && dense(p.rejected.mask, p.rejected.steps, V) && aligned_to(a.grad[0], 16) &&
+                    aligned_to(a.grad[1], 16);
+  const long long n = p.pairs * (p.chosen.steps > p.rejected.steps ? p.chosen.steps : p.rejected.steps);
+  if (n == 0) return SDEH_OK;
+  const int v = wide ? V : 1;
+  long long blocks = (n + (long long)kThreads * v - 1) / ((long long)kThreads * v);
+  if (blocks > 1024) blocks = 1024;
+  grad_strides(a, blocks, kThreads, v);
+  if (wide)
+    hipLaunchKernelGGL((preference_grad_kernel<T, V>), dim3((unsigned)blocks, 2), dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((preference_grad_kernel<T, 1>), dim3((unsigned)blocks, 2), dim3(kThreads), 0, stream, a);
+  return hipGetLastError() == hipSuccess ? SDEH_OK : SDEH_ERR_HIP;
+}
+
+template <typename T>
+int launch_preference_t(PreferenceArgs a, hipStream_t stream) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const SdehPreferenceLoss& p = a.p;
+  const long long longest = p.chosen.steps > p.rejected.steps ? p.chosen.steps : p.rejected.steps;
+  const bool wide = dense_side(p.chosen, V) && dense_side(p.rejected, V);
+  if (p.pairs * (p.chosen.steps + p.rejected.steps) <= kPreferenceSmall && longest <= kShortRow && p.pairs <= kSmallThreads) {
+    const bool grad_wide = wide && aligned_to(a.grad[0], 16) && aligned_to(a.grad[1], 16);
+    grad_strides(a, 1, kSmallThreads, grad_wide ? V : 1);
+    if (grad_wide)
+      hipLaunchKernelGGL((preference_small_kernel<T, V>), dim3(1), dim3(kSmallThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL((preference_small_kernel<T, 1>), dim3(1), dim3(kSmallThreads), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? SDEH_OK : SDEH_ERR_HIP;
+  }
+  a.chunk = (longest + a.splits - 1) / a.splits;
+  a.chunk = (a.chunk + 15) / 16 * 16;
+  if (longest <= kShortRow) {
+    const long long blocks = (2 * p.pairs + kThreads / 64 - 1) / (kThreads / 64);
+    const dim3 grid((unsigned)(blocks > 8192 ? 8192 : blocks));
+    if (wide)
+      hipLaunchKernelGGL((preference_short_kernel<T, V>), grid, dim3(kThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL((preference_short_kernel<T, 1>), grid, dim3(kThreads), 0, stream, a);
+  } else {
+    const long long blocks = 2 * p.pairs * a.splits;
+    if (blocks > 0x7FFFFFFFll) return SDEH_ERR_UNSUPPORTED;
+    if (wide)
+      hipLaunchKernelGGL((preference_sum_kernel<T, V>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL((preference_sum_kernel<T, 1>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+  }
+  const long long per = a.splits == 1 ? kThreads : kThreads / 64;
+  long long pair_blocks = (p.pairs + per - 1) / per;
+  a.n_pair_blocks = (int)(pair_blocks > kPairBlocks ? kPairBlocks : pair_blocks);
+  hipLaunchKernelGGL(preference_pair_kernel, dim3(a.n_pair_blocks), dim3(kThreads), 0, stream, a);
+  if (a.n_pair_blocks > 1) hipLaunchKernelGGL(preference_final_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+  if (hipGetLastError() != hipSuccess) return SDEH_ERR_HIP;
+  if (a.grad[0] == nullptr) return SDEH_OK;
+  a.slopes = a.out + 2 + 2 * p.pairs;
+  return launch_spread_t<T>(a, stream);
+}
+
+}  // namespace
+
+// scratch: partial losses, sums, counts
+long long preference_scratch_floats(const SdehPreferenceLoss& p) { return kPairBlocks * 4ll + 8ll * p.pairs * preference_splits(p); }
+
+int launch_preference_loss(const SdehPreferenceLoss& p, float* scratch, float grad_factor, float* out, void* grad_c, void* grad_r,
+                           hipStream_t stream) {
+  PreferenceArgs a{};
+  a.p = p;
+  a.splits = preference_splits(p);
+  a.part = reinterpret_cast<double*>(scratch);
+  a.sum = a.part + 2 * kPairBlocks;
+  a.count = reinterpret_cast<long long*>(a.sum + 2 * p.pairs * a.splits);
+  a.out = out;
+  a.grad_factor = grad_factor;
+  a.grad[0] = grad_c;
+  a.grad[1] = grad_r;
+  return p.dtype == SDEH_F32 ? launch_preference_t<float>(a, stream)
+                             : p.dtype == SDEH_BF16 ? launch_preference_t<bf16_t>(a, stream) : launch_preference_t<f16_t>(a, stream);
+}
+
+int launch_preference_grad(const SdehPreferenceLoss& p, const float* out, const float* grad_scale, float grad_factor, void* grad_c, void* grad_r,
+                           hipStream_t stream) {
+  PreferenceArgs a{};
+  a.p = p;
+  a.slopes = out + 2 + 2 * p.pairs;
+  a.grad_scale = grad_scale;
+  a.grad_factor = grad_factor;
+  a.grad[0] = grad_c;
+  a.grad[1] = grad_r;
+  return p.dtype == SDEH_F32 ? launch_spread_t<float>(a, stream)
+                             : p.dtype == SDEH_BF16 ? launch_spread_t<bf16_t>(a, stream) : launch_spread_t<f16_t>(a, stream);
+}
+
+}  // namespace sdeh

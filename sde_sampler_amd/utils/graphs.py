@@ -36,6 +36,7 @@ from typing import Callable, Iterable
 import torch
 
 from sde_sampler_amd import _lib as L
+from sde_sampler_amd.utils.optim import AdamW
 
 __all__ = ["GraphedTrainStep", "GraphedEval"]
 
@@ -50,7 +51,8 @@ class GraphedTrainStep:
     loss_fn          () -> scalar loss tensor; may draw samples with torch's device generator, must not synchronise and must
                      only read tensors that stay alive (parameters, `ts`, buffers of the prior / target)
     losses           the loss objects `loss_fn` calls (their `rng_counter` / `graph_safe` are set here)
-    optimizer        for Adam/AdamW pass `capturable=True`
+    optimizer        for torch's Adam/AdamW pass `capturable=True`; `utils.optim.AdamW` takes the guard's decision itself (no snapshot of the
+                     parameters and moments, nothing to put back) and clips by its own `max_grad_norm`
     reduce_gradients optional () -> None right after backward, BEFORE the finite-gradient guard (data parallelism:
                      `lambda: all_reduce_gradients(params)`): the accept / reject decision is then taken on the REDUCED gradients
                      and is the same on every rank -- a NaN from another rank, or the disagreement poison of
@@ -82,6 +84,7 @@ class GraphedTrainStep:
         self.guard, self.max_loss = guard, max_loss
         self.n_skipped = torch.zeros((), dtype=torch.int64, device=self.device)
         self._params = [p for g in optimizer.param_groups for p in g["params"] if p.requires_grad]
+        self._skips_itself = isinstance(optimizer, AdamW)
         self._snap: list[torch.Tensor] | None = None
         self._table, self._table_key = None, None
 
@@ -95,7 +98,7 @@ class GraphedTrainStep:
             # follows one step later: keep stepping eagerly until a step has left it alone (warmup <= 1 used to rebuild it
             # inside the capture).  These are real optimisation steps, like the warm-up's.
             extra = 0
-            while self.guard and not self._table_ready():
+            while self.guard and not self._skips_itself and not self._table_ready():
                 if extra == 4:
                     raise RuntimeError("GraphedTrainStep(guard=True): the optimizer state keeps changing its tensors from step to step; "
                                        "it cannot be captured")
@@ -184,6 +187,11 @@ class GraphedTrainStep:
                 torch._foreach_copy_(grads, [c.view_as(g) for c, g in zip(flat.split([g.numel() for g in grads]), grads)])
             if self._after_backward is not None:
                 self._after_backward()
+            if self._skips_itself:
+                self.optimizer.step(ok=ok)
+                self.n_skipped += (~ok).reshape(()).to(torch.int64)
+                self.counter.add_(1)
+                return value.detach()
             with torch.no_grad():
                 tensors = [t.detach() for t in self._guarded()]
                 if self._snap is None or len(self._snap) != len(tensors):  # (re)built while the optimizer state appears (warm-up)
