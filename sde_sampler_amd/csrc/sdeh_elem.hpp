@@ -29,6 +29,22 @@ __device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&x)[V
   *reinterpret_cast<Pack<T, V>*>(p) = k;
 }
 
+// 16 bytes as they were loaded, and their values: loads that run ahead of their use stay in this form (a value unpacked where it is loaded is waited for
+// there)
+typedef unsigned Raw __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ Raw load_raw(const T* p) {
+  return *reinterpret_cast<const Raw*>(p);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Raw& r, float (&x)[V]) {
+  const Pack<T, V> k = __builtin_bit_cast(Pack<T, V>, r);
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = static_cast<float>(k.v[i]);
+}
+
 // one element of a tensor whose type is known at run time
 __device__ __forceinline__ float load_as(const void* p, int dtype, long long i) {
   if (dtype == SDEH_F32) return static_cast<const float*>(p)[i];

@@ -188,13 +188,13 @@ namespace {
 // every workgroup of the main pass adds up again.  No atomics, no last-workgroup ticket: results do not depend on the order of workgroups and
 // nothing has to be cleared between calls.
 // -------------------------------------------------------------------------------------------------------------------------------------------
-constexpr int kCountBlocks = 512, kPolicyBlocks = 2048, kSmallThreads = 1024;
+constexpr int kCountBlocks = 1024, kPolicyBlocks = 2048, kSmallThreads = 1024;
 
 struct PolicyArgs {
   SdehPolicyLoss p;
   long long n;          // rows * steps
-  long long d_row, d_col;  // (rows, steps) that one iteration of the grid moves an entry by
-  double log_hi, log_lo, log_dual;
+  double log_hi, log_lo, log_dual;     // the borders' logarithms,
+  float log_hi_f, log_lo_f, log_dual_f;  // and rounded
   float hi, lo, dual, kl_coef;
   const float* grad_scale;
   float grad_factor;
@@ -204,7 +204,6 @@ struct PolicyArgs {
   long long* part_n;    // [kCountBlocks]
   double* part;         // [kPolicyBlocks][4]
   int n_count, n_part;  // workgroups of the two passes
-  bool flat_advantage;  // fp32, laid out like the other planes
 };
 
 __device__ __forceinline__ bool needs_counts(const PolicyArgs& a) { return a.p.mask.data != nullptr && a.p.reduction != SDEH_REDUCE_SUM; }
@@ -221,9 +220,9 @@ __device__ __forceinline__ int count_span(const uint8_t* m, long long n, long lo
   for (long long i = me; i < head; i += team) c += m[i] != 0;
 #pragma unroll 4
   for (long long i = me; i < packs; i += team) {
-    const Pack<uint8_t, 16> k = *reinterpret_cast<const Pack<uint8_t, 16>*>(m + head + 16 * i);
+    const Pack<unsigned, 4> k = *reinterpret_cast<const Pack<unsigned, 4>*>(m + head + 16 * i);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) c += k.v[j] != 0;
+    for (int j = 0; j < 4; ++j) c += __popc((((k.v[j] & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | k.v[j]) & 0x80808080u);  // (bit 7 of every byte that is not 0)
   }
   for (long long i = head + 16 * packs + me; i < n; i += team) c += m[i] != 0;
   return c;
@@ -275,176 +274,298 @@ __device__ __forceinline__ double common_weight(const PolicyArgs& a, int n_count
   return 1.0 / (double)(n > 0 ? n : 1);
 }
 
-// exp(-k) - 1 + k and its slope 1 - exp(-k).  Below |k| = 1/2 by its series (the difference would lose the digits that exp(-k) and 1 - k share):
-// k^2 (1/2! - k/3! + ... + k^8/10!), the first term left out is below 1e-10 of the sum.
-__device__ __forceinline__ float kl3(float k, float& slope) {
-  const float e = expf(-k);
-  const float far = (e - 1.0f) + k;
-  float s = 2.7557319e-7f;
-  s = fmaf(-k, s, 2.7557319e-6f);
-  s = fmaf(-k, s, 2.4801587e-5f);
-  s = fmaf(-k, s, 1.9841270e-4f);
-  s = fmaf(-k, s, 1.3888889e-3f);
-  s = fmaf(-k, s, 8.3333333e-3f);
-  s = fmaf(-k, s, 4.1666667e-2f);
-  s = fmaf(-k, s, 1.6666667e-1f);
-  s = fmaf(-k, s, 0.5f);
-  const float near = k * k * s;
-  const bool small = fabsf(k) < 0.5f;
-  slope = small ? k - near : 1.0f - e;
-  return small ? near : far;
-}
+// exp(x) from the hardware's 2^y (one unit in the last place; results below 2^-126 become 0).  y = x log2(e) is rounded: off by at most
+// (2 + 1.3 |x|) 2^-24 of itself, and a ratio's |x| is seldom above 1.  Two instructions where the library's takes thirteen.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
 
 struct PolicySums {
   double policy, kl;
-  long long clipped, valid;
+  unsigned clipped, valid;  // (a thread meets fewer than 2^32 entries)
 };
 
-// All entries, V neighbours a thread.  V > 1: every plane is contiguous and aligned; V = 1: any strides.
-template <typename T, int V, int NT>
-__device__ __forceinline__ PolicySums policy_pass(const PolicyArgs& a, double w_common) {
+// The KL term of V entries, k = log_prob - ref: value and slope.  (What does not depend on the entry is decided outside the loops over entries here and
+// below: with these decisions inside, the compiler spent more instructions on branches than on the mathematics.)
+//   k3: exp(-k) - 1 + k and 1 - exp(-k).  Up to |k| = 1 from a polynomial (the difference would lose the digits that exp(-k) and 1 - k share):
+//   (exp(-k) - 1 + k) / k^2 through its eight Chebyshev nodes of [-1, 1], off by less than 2e-08 of itself with these coefficients.
+template <int V>
+__device__ __forceinline__ void kl_terms(int kind, const float (&x)[V], const float (&q)[V], float (&kl)[V], float (&slope)[V]) {
+  if (kind == SDEH_KL_3) {
+    bool far = false;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float k = x[j] - q[j];
+      float s = -2.80628024e-06f;
+      s = fmaf(k, s, 2.53585131e-05f);
+      s = fmaf(k, s, -0.000198381022f);
+      s = fmaf(k, s, 0.00138853968f);
+      s = fmaf(k, s, -0.00833333936f);
+      s = fmaf(k, s, 0.041666735f);
+      s = fmaf(k, s, -0.166666672f);
+      s = fmaf(k, s, 0.5f);
+      kl[j] = k * k * s;
+      slope[j] = k - kl[j];
+      far |= !(fabsf(k) <= 1.0f);
+    }
+    if (far) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float k = x[j] - q[j], e = fast_exp(-k), far_kl = (e - 1.0f) + k, far_slope = 1.0f - e;
+        const bool near = fabsf(k) <= 1.0f;
+        kl[j] = near ? kl[j] : far_kl;
+        slope[j] = near ? slope[j] : far_slope;
+      }
+    }
+  } else if (kind == SDEH_KL_2) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      slope[j] = x[j] - q[j];
+      kl[j] = 0.5f * slope[j] * slope[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      kl[j] = x[j] - q[j];
+      slope[j] = 1.0f;
+    }
+  }
+}
+
+// V entries from their values: adds to `sums`, returns the gradients (without the loss's own scale).  MASKED: `ok` has a bit for each valid entry.
+//
+// Which side of a border the ratio lies on has to be right to the last bit of delta = x - o, whose fp32 value d is rounded.  Rounding is monotonic, so
+// d > border (rounded) says delta > border (exactly) and d < border the opposite; only where they are equal are the 64-bit numbers compared, and d is
+// moved to its neighbour beyond the border where delta lies beyond.  Then fp32 comparisons are right, and nothing but d depends on that rare branch.
+template <int V, bool MASKED>
+__device__ __forceinline__ void policy_entries(const PolicyArgs& a, const float (&x)[V], const float (&o)[V], const float (&q)[V], const float (&adv)[V],
+                                               const float (&w)[V], unsigned ok, bool has_ref, bool row_weight, PolicySums& sums, float (&g)[V]) {
+  float d[V];
+  bool close = false;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    d[k] = adv[k] == 0.0f ? 0.0f : x[k] - o[k];  // (no advantage: nothing, whatever the ratio; 0 is never beyond a border)
+    close |= (d[k] == (adv[k] > 0.0f ? a.log_hi_f : a.log_lo_f)) | (d[k] == a.log_dual_f);
+  }
+  if (close) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const double delta = (double)x[k] - (double)o[k];
+      if (adv[k] > 0.0f && d[k] == a.log_hi_f && delta > a.log_hi) d[k] = nextafterf(d[k], HUGE_VALF);
+      if (adv[k] < 0.0f && d[k] == a.log_lo_f && delta < a.log_lo) d[k] = nextafterf(d[k], -HUGE_VALF);
+      if (adv[k] < 0.0f && d[k] == a.log_dual_f && delta > a.log_dual) d[k] = nextafterf(d[k], HUGE_VALF);
+    }
+  }
+  float surrogate[V], slope[V], kl[V];
+  unsigned clips = 0;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const bool up = adv[k] > 0.0f, over = !up & (d[k] > a.log_dual_f);
+    const bool beyond = (up ? d[k] : -d[k]) > (up ? a.log_hi_f : -a.log_lo_f), clipped = beyond | over;
+    const float bound = over ? a.dual : up ? a.hi : a.lo, r = fast_exp(d[k]);
+    surrogate[k] = -adv[k] * (clipped ? bound : r);
+    slope[k] = clipped ? 0.0f : surrogate[k];
+    kl[k] = 0.0f;
+    if (MASKED)
+      clips |= clipped ? 1u << k : 0u;
+    else
+      sums.clipped += clipped;
+  }
+  if (has_ref) {
+    float kl_slope[V];
+    kl_terms<V>(a.p.kl, x, q, kl, kl_slope);
+#pragma unroll
+    for (int k = 0; k < V; ++k) slope[k] = fmaf(a.kl_coef, kl_slope[k], slope[k]);
+  }
+  if (row_weight) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      surrogate[k] *= w[k];
+      kl[k] *= w[k];
+    }
+  }
+  float policy = 0.0f, kls = 0.0f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const bool in = !MASKED || (ok >> k & 1u) != 0u;
+    policy += in ? surrogate[k] : 0.0f;
+    kls += in ? kl[k] : 0.0f;
+    g[k] = in ? slope[k] * w[k] : 0.0f;
+  }
+  if (MASKED) sums.clipped += __popc(clips & ok);
+  sums.valid += MASKED ? __popc(ok) : V;
+  sums.policy += (double)policy;
+  sums.kl += (double)kls;
+}
+
+// bit k of the result: byte k of the word is not 0
+__device__ __forceinline__ unsigned byte_bits(unsigned m) {
+  const unsigned t = (((m & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | m) & 0x80808080u;
+  return (t >> 7 & 1u) | (t >> 14 & 2u) | (t >> 21 & 4u) | (t >> 28 & 8u);
+}
+
+// what a pass needs throughout
+struct PolicyView {
+  bool has_ref, row_weight;
+  float w_all, factor;
+};
+
+__device__ __forceinline__ PolicyView policy_view(const PolicyArgs& a, double w_common) {
+  PolicyView v;
+  v.has_ref = a.p.ref_log_prob.data != nullptr;
+  v.row_weight = a.p.reduction == SDEH_REDUCE_ROWS;
+  // a row's weight is taken from its count where there is a mask; without one all rows have as many entries
+  v.w_all = (float)(v.row_weight && a.p.mask.data == nullptr ? w_common / (double)a.p.steps : w_common);
+  v.factor = a.grad_factor * (a.grad_scale != nullptr ? *a.grad_scale : 1.0f);
+  return v;
+}
+
+// one entry of planes with any strides
+template <typename T>
+__device__ __forceinline__ void policy_one(const PolicyArgs& a, const PolicyView& v, long long row, long long col, PolicySums& sums) {
+  const SdehPolicyLoss& p = a.p;
+  const auto at = [&](const SdehPlane& q) { return (float)static_cast<const T*>(q.data)[row * q.row_stride + col * q.step_stride]; };
+  float g[1] = {0.0f};
+  if (p.mask.data == nullptr || static_cast<const uint8_t*>(p.mask.data)[row * p.mask.row_stride + col * p.mask.step_stride] != 0) {
+    const float x[1] = {at(p.log_prob)}, o[1] = {p.old_log_prob.data != nullptr ? at(p.old_log_prob) : 0.0f}, q[1] = {v.has_ref ? at(p.ref_log_prob) : 0.0f};
+    const float adv[1] = {load_as(p.advantage.data, p.advantage_dtype, row * p.advantage.row_stride + col * p.advantage.step_stride)};
+    const float w[1] = {v.row_weight && p.mask.data != nullptr ? v.w_all / (float)a.row_count[row] : v.w_all};
+    policy_entries<1, false>(a, x, o, q, adv, w, 1u, v.has_ref, v.row_weight, sums, g);
+  }
+  if (a.grad != nullptr) static_cast<T*>(a.grad)[row * p.steps + col] = static_cast<T>(g[0] * v.factor);
+}
+
+// All entries.  V > 1: every plane is contiguous and aligned, V neighbours a thread; V = 1: any strides.  ROW: the entry's row matters (an advantage or a
+// weight of its own); without it the entries are one stream.
+//
+// The grid goes over the entries in rounds, a tile of NT V neighbours a workgroup.  With rows that end early, a workgroup that met the same place of
+// every row would have nothing but valid entries, another nothing but padding, wherever a round's length is near a multiple of `steps`: the workgroups
+// change places from round to round.
+template <typename T, int V, int NT, bool ROW>
+__device__ __forceinline__ PolicySums policy_pass(const PolicyArgs& a) {
   PolicySums sums{0.0, 0.0, 0, 0};
   const SdehPolicyLoss& p = a.p;
-  const T* lp = static_cast<const T*>(p.log_prob.data);
-  const T* old = static_cast<const T*>(p.old_log_prob.data);
-  const T* ref = static_cast<const T*>(p.ref_log_prob.data);
-  const uint8_t* mask = static_cast<const uint8_t*>(p.mask.data);
-  T* grad = static_cast<T*>(a.grad);
-  const bool row_adv = V > 1 && p.advantage.step_stride == 0;
-  const bool flat_adv = V > 1 && a.flat_advantage;
-  const bool row_weight = p.reduction == SDEH_REDUCE_ROWS;
-  const float w_all = (float)w_common, w_dense = row_weight ? (float)(w_common / (double)p.steps) : w_all;
-  const float factor = a.grad_factor * (a.grad_scale != nullptr ? *a.grad_scale : 1.0f);
-  const long long stride = (long long)gridDim.x * NT * V;
-  long long i = ((long long)blockIdx.x * NT + threadIdx.x) * V;
-  if (i >= a.n) return sums;
-  long long row = i / p.steps, col = i - row * p.steps;
-  for (; i < a.n; i += stride) {
-    const int live = a.n - i < V ? (int)(a.n - i) : V;
-    bool ok[V];
-    int any = 0;
-    if (mask == nullptr) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) ok[k] = k < live;
-      any = 1;
-    } else if (V > 1 && live == V) {
-      const Pack<uint8_t, V> m = *reinterpret_cast<const Pack<uint8_t, V>*>(mask + i);
-#pragma unroll
-      for (int k = 0; k < V; ++k) any |= ok[k] = m.v[k] != 0;
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        ok[k] = k < live && mask[V > 1 ? i + k : row * p.mask.row_stride + col * p.mask.step_stride] != 0;
-        any |= ok[k];
-      }
+  const long long me = (long long)blockIdx.x * NT + threadIdx.x, body = a.n / V * V;
+  const unsigned shift = (unsigned)((unsigned long long)gridDim.x * 382u / 1000u) | 1u;
+  const auto place = [&](long long round) {  // first entry of this workgroup's tile
+    const unsigned at = (unsigned)((blockIdx.x + (unsigned long long)round * shift) % gridDim.x);
+    return (round * gridDim.x + at) * ((long long)NT * V);
+  };
+  const long long rounds = (body + (long long)gridDim.x * NT * V - 1) / ((long long)gridDim.x * NT * V);
+  if constexpr (V == 1) {
+    const PolicyView v = policy_view(a, common_weight<NT>(a, a.n_count));
+    for (long long round = 0; round < rounds; ++round) {
+      const long long i = place(round) + threadIdx.x;
+      if (i < body) policy_one<T>(a, v, i / p.steps, i % p.steps, sums);
     }
-    float g[V];
+  } else {
+    const T* lp = static_cast<const T*>(p.log_prob.data);
+    const T* old = static_cast<const T*>(p.old_log_prob.data);
+    const T* ref = static_cast<const T*>(p.ref_log_prob.data);
+    const uint8_t* mask = static_cast<const uint8_t*>(p.mask.data);
+    T* grad = static_cast<T*>(a.grad);
+    const bool row_adv = p.advantage.step_stride == 0;
+    constexpr unsigned kAll = (1u << V) - 1u;
+    // Two vectors ahead its mask, one vector ahead its values are on their way: what is loaded depends on the mask, and four or five waves of this many
+    // registers do not cover both latencies by themselves.
+    const auto load_mask = [&](long long at) {
+      Pack<unsigned, V / 4> m{};
+      if (mask != nullptr && at < body) m = *reinterpret_cast<const Pack<unsigned, V / 4>*>(mask + at);
+      return m;
+    };
+    const auto valid = [&](const Pack<unsigned, V / 4>& m, long long at) {
+      if (at >= body) return 0u;
+      if (mask == nullptr) return kAll;
+      unsigned ok = byte_bits(m.v[0]);
+      if constexpr (V == 8) ok |= byte_bits(m.v[1]) << 4;
+      return ok;
+    };
+    // (absent planes are read from log_prob's place, so that no load waits behind a branch, and count as 0)
+    const T* old_at = old != nullptr ? old : lp;
+    const T* ref_at = ref != nullptr ? ref : lp;
+    Raw next_x{}, next_o{}, next_q{}, next_a[V / 4]{};
+    const auto load_values = [&](long long at, unsigned ok) {
+      if (ok != 0u) {  // (a stretch of padding is neither read nor computed)
+        next_x = load_raw(lp + at);
+        next_o = load_raw(old_at + at);
+        next_q = load_raw(ref_at + at);
+        if constexpr (!ROW) {  // (the advantage is fp32 and laid out like the rest)
 #pragma unroll
-    for (int k = 0; k < V; ++k) g[k] = 0.0f;
-    if (any) {  // (a stretch of padding is neither read nor computed)
-      float x[V], o[V], q[V], adv[V];
-      if (V > 1 && live == V) {
-        load_pack<T, V>(lp + i, x);
-        if (old != nullptr) load_pack<T, V>(old + i, o);
-        if (ref != nullptr) load_pack<T, V>(ref + i, q);
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const bool in = k < live;
-          x[k] = in ? (float)lp[V > 1 ? i + k : row * p.log_prob.row_stride + col * p.log_prob.step_stride] : 0.0f;
-          if (old != nullptr) o[k] = in ? (float)old[V > 1 ? i + k : row * p.old_log_prob.row_stride + col * p.old_log_prob.step_stride] : 0.0f;
-          if (ref != nullptr) q[k] = in ? (float)ref[V > 1 ? i + k : row * p.ref_log_prob.row_stride + col * p.ref_log_prob.step_stride] : 0.0f;
+          for (int k = 0; k < V / 4; ++k) next_a[k] = load_raw(static_cast<const float*>(p.advantage.data) + at + 4 * k);
         }
       }
-      if (flat_adv && live == V) {
-        if constexpr (V > 4) {
-          float half[4];
+    };
+    const long long mine = (long long)threadIdx.x * V;
+    long long start = place(0), start_next = rounds > 1 ? place(1) : body;
+    unsigned ok_next = valid(load_mask(start + mine), start + mine);
+    load_values(start + mine, ok_next);
+    Pack<unsigned, V / 4> m = load_mask(start_next + mine);
+    const PolicyView v = policy_view(a, common_weight<NT>(a, a.n_count));
+    const bool count = v.row_weight && mask != nullptr;
+    for (long long round = 0; round < rounds; ++round) {
+      const long long i = start + mine;
+      const unsigned ok = ok_next;
+      float x[V], o[V], q[V], adv[V], w[V];
+      unpack<T, V>(next_x, x);
+      unpack<T, V>(next_o, o);
+      unpack<T, V>(next_q, q);
+      if constexpr (!ROW) {
 #pragma unroll
-          for (int j = 0; j < V; j += 4) {
-            load_pack<float, 4>(static_cast<const float*>(p.advantage.data) + i + j, half);
+        for (int k = 0; k < V; ++k) adv[k] = __uint_as_float(next_a[k / 4][k % 4]);
+      }
+      ok_next = valid(m, start_next + mine);
+      load_values(start_next + mine, ok_next);
+      long long row = 0, col = 0;
+      if constexpr (ROW) {  // (the tile's place by 64-bit arithmetic of the whole wave, the thread's in it by 32-bit arithmetic)
+        const long long r0 = start / p.steps;
+        const unsigned t = (unsigned)(start - r0 * p.steps) + (unsigned)mine, r = t / (unsigned)p.steps;
+        row = r0 + r;
+        col = t - r * (unsigned)p.steps;
+      }
+      start = start_next;
+      start_next = round + 2 < rounds ? place(round + 2) : body;
+      m = load_mask(start_next + mine);
+      float g[V];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) adv[j + k] = half[k];
+      for (int k = 0; k < V; ++k) g[k] = 0.0f;
+      if (ok != 0u) {
+        if (old == nullptr) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) o[k] = 0.0f;
+        }
+        if constexpr (!ROW) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) w[k] = v.w_all;
+        } else if (row_adv && col + V <= p.steps) {  // (one row)
+          const float A = load_as(p.advantage.data, p.advantage_dtype, row * p.advantage.row_stride);
+          const float wr = count ? v.w_all / (float)a.row_count[row] : v.w_all;
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            adv[k] = A;
+            w[k] = wr;
           }
         } else {
-          load_pack<float, V>(static_cast<const float*>(p.advantage.data) + i, adv);
-        }
-      }
-      float w[V];
-      {
-        long long r = row, c = col;
-        float a_row = 0.0f, w_row = w_dense;
-        bool fresh = true;
+          long long r = row, c = col;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          if (fresh && k < live) {
-            if (row_adv) a_row = load_as(p.advantage.data, p.advantage_dtype, r * p.advantage.row_stride);
-            if (row_weight && mask != nullptr) w_row = w_all / (float)a.row_count[r];  // (only entries of rows that have one are weighed)
-          }
-          adv[k] = row_adv                    ? a_row
-                   : flat_adv && live == V ? adv[k]
-                   : k < live ? load_as(p.advantage.data, p.advantage_dtype, r * p.advantage.row_stride + c * p.advantage.step_stride) : 0.0f;
-          w[k] = w_row;
-          fresh = ++c == p.steps;
-          if (fresh) {
-            c = 0;
-            ++r;
+          for (int k = 0; k < V; ++k) {
+            adv[k] = load_as(p.advantage.data, p.advantage_dtype, r * p.advantage.row_stride + c * p.advantage.step_stride);
+            w[k] = count ? v.w_all / (float)a.row_count[r] : v.w_all;  // (a row without a valid entry: nothing of it is added)
+            if (++c == p.steps) {
+              c = 0;
+              ++r;
+            }
           }
         }
+        if (ok == kAll)
+          policy_entries<V, false>(a, x, o, q, adv, w, ok, v.has_ref, v.row_weight, sums, g);
+        else
+          policy_entries<V, true>(a, x, o, q, adv, w, ok, v.has_ref, v.row_weight, sums, g);
       }
-      float s_policy = 0.0f, s_kl = 0.0f;
+      if (grad != nullptr) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const double delta = old != nullptr ? (double)x[k] - (double)o[k] : (double)x[k];
-        const bool over = delta > a.log_hi, under = delta < a.log_lo;
-        const float A = adv[k];
-        bool clipped = (A > 0.0f && over) || (A < 0.0f && under);
-        float bound = over ? a.hi : a.lo;
-        if (A < 0.0f && delta > a.log_dual) {
-          clipped = true;
-          bound = a.dual;
-        }
-        const float used = clipped ? bound : expf((float)delta);
-        const float surrogate = A == 0.0f ? 0.0f : -A * used;
-        float slope = clipped ? 0.0f : surrogate;
-        float kl = 0.0f;
-        if (ref != nullptr) {
-          const float d = (float)((double)x[k] - (double)q[k]);
-          float kl_slope;
-          if (p.kl == SDEH_KL_3) {
-            kl = kl3(d, kl_slope);
-          } else if (p.kl == SDEH_KL_2) {
-            kl = 0.5f * d * d;
-            kl_slope = d;
-          } else {
-            kl = d;
-            kl_slope = 1.0f;
-          }
-          slope = fmaf(a.kl_coef, kl_slope, slope);
-        }
-        s_policy += ok[k] ? (row_weight ? surrogate * w[k] : surrogate) : 0.0f;
-        s_kl += ok[k] ? (row_weight ? kl * w[k] : kl) : 0.0f;
-        sums.clipped += ok[k] && clipped;
-        sums.valid += ok[k];
-        g[k] = ok[k] ? slope * w[k] * factor : 0.0f;
-      }
-      sums.policy += (double)s_policy;
-      sums.kl += (double)s_kl;
-    }
-    if (grad != nullptr) {
-      if (V > 1 && live == V) {
-        store_pack<T, V>(grad + i, g);
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (k < live) grad[i + k] = static_cast<T>(g[k]);
+        for (int k = 0; k < V; ++k) g[k] *= v.factor;
+        if (i < body) store_pack<T, V>(grad + i, g);
       }
     }
-    row += a.d_row;
-    col += a.d_col;
-    if (col >= p.steps) {
-      col -= p.steps;
-      ++row;
-    }
+    if (me < a.n - body) policy_one<T>(a, v, (body + me) / p.steps, (body + me) % p.steps, sums);  // (less than a vector is left)
   }
   return sums;
 }
@@ -468,13 +589,12 @@ __global__ __launch_bounds__(NT) void policy_count_kernel(PolicyArgs a) {
   count_pass<NT>(a);
 }
 
-template <typename T, int V>
+template <typename T, int V, bool ROW>
 __global__ __launch_bounds__(kThreads) void policy_kernel(PolicyArgs a) {
-  const double w = common_weight<kThreads>(a, a.n_count);
-  const PolicySums s = policy_pass<T, V, kThreads>(a, w);
+  const PolicySums s = policy_pass<T, V, kThreads, ROW>(a);
   if (a.out == nullptr) return;
   const double policy = block_sum<kThreads>(s.policy), kl = block_sum<kThreads>(s.kl);
-  const long long clipped = block_sum<kThreads>(s.clipped), valid = block_sum<kThreads>(s.valid);
+  const long long clipped = block_sum<kThreads>((long long)s.clipped), valid = block_sum<kThreads>((long long)s.valid);
   if (threadIdx.x == 0) {
     double* o = a.part + 4 * blockIdx.x;
     o[0] = policy;
@@ -502,11 +622,10 @@ __global__ __launch_bounds__(kSmallThreads) void policy_small_kernel(PolicyArgs 
     __threadfence_block();
     __syncthreads();
   }
-  const double w = common_weight<kSmallThreads>(a, 1);
-  const PolicySums s = policy_pass<T, V, kSmallThreads>(a, w);
+  const PolicySums s = policy_pass<T, V, kSmallThreads, true>(a);
   if (a.out == nullptr) return;
   const double policy = block_sum<kSmallThreads>(s.policy), kl = block_sum<kSmallThreads>(s.kl);
-  const long long clipped = block_sum<kSmallThreads>(s.clipped), valid = block_sum<kSmallThreads>(s.valid);
+  const long long clipped = block_sum<kSmallThreads>((long long)s.clipped), valid = block_sum<kSmallThreads>((long long)s.valid);
   if (threadIdx.x == 0) policy_result(a, policy, kl, (double)clipped, (double)valid);
 }
 
@@ -523,17 +642,15 @@ int launch_policy_t(PolicyArgs a, bool reuse_counts, hipStream_t stream) {
   const bool adv_ok = p.advantage.step_stride == 0 || p.advantage.step_stride == 1;
   const bool wide = dense(p.log_prob, p.steps, 16) && dense(p.old_log_prob, p.steps, 16) && dense(p.ref_log_prob, p.steps, 16) &&
                     dense(p.mask, p.steps, V) && adv_ok && aligned_to(a.grad, 16);
-  a.flat_advantage = wide && p.advantage_dtype == SDEH_F32 && dense(p.advantage, p.steps, 16);
+  const bool stream_only = wide && p.advantage_dtype == SDEH_F32 && dense(p.advantage, p.steps, 16) && (p.reduction != SDEH_REDUCE_ROWS || p.mask.data == nullptr);
   const int v = wide ? V : 1;
   const bool small = a.n <= kPolicySmall;
   const int nt = small ? kSmallThreads : kThreads;
-  long long blocks = (a.n + (long long)nt * v - 1) / ((long long)nt * v);
-  blocks = small ? 1 : blocks > kPolicyBlocks ? kPolicyBlocks : blocks;
-  const long long stride = blocks * nt * v;
-  a.d_row = p.steps > 0 ? stride / p.steps : 0;
-  a.d_col = p.steps > 0 ? stride % p.steps : 0;
+  const long long tiles = (a.n + (long long)nt * v - 1) / ((long long)nt * v), most = wide && V == 8 ? kPolicyBlocks / 2 : kPolicyBlocks;
+  const long long blocks = small || tiles == 0 ? 1 : tiles > most ? most : tiles;  // (as many as are resident at once)
   a.n_part = (int)blocks;
   if (small) {
+    a.n_count = 1;
     if (wide)
       hipLaunchKernelGGL((policy_small_kernel<T, V>), dim3(1), dim3(kSmallThreads), 0, stream, a);
     else
@@ -549,10 +666,12 @@ int launch_policy_t(PolicyArgs a, bool reuse_counts, hipStream_t stream) {
     else
       hipLaunchKernelGGL(policy_count_kernel<kThreads>, dim3(a.n_count), dim3(kThreads), 0, stream, a);
   }
-  if (wide)
-    hipLaunchKernelGGL((policy_kernel<T, V>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+  if (stream_only)
+    hipLaunchKernelGGL((policy_kernel<T, V, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+  else if (wide)
+    hipLaunchKernelGGL((policy_kernel<T, V, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((policy_kernel<T, 1>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((policy_kernel<T, 1, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
   if (a.out != nullptr) hipLaunchKernelGGL(policy_final_kernel, dim3(1), dim3(kThreads), 0, stream, a);
   return hipGetLastError() == hipSuccess ? SDEH_OK : SDEH_ERR_HIP;
 }
@@ -570,6 +689,9 @@ int launch_policy_loss(const SdehPolicyLoss& p, float* scratch, int reuse_counts
   a.log_hi = log1p(p.clip_high);
   a.log_lo = p.clip_low < 1.0 ? log1p(-p.clip_low) : -HUGE_VAL;
   a.log_dual = p.dual_clip > 0.0 ? log(p.dual_clip) : HUGE_VAL;
+  a.log_hi_f = (float)a.log_hi;
+  a.log_lo_f = (float)a.log_lo;
+  a.log_dual_f = (float)a.log_dual;
   a.hi = (float)(1.0 + p.clip_high);
   a.lo = (float)(1.0 - p.clip_low);
   a.dual = (float)p.dual_clip;
