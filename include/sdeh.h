@@ -635,9 +635,9 @@ typedef struct {
   double lr, beta1, beta2, eps, weight_decay;
   const float* lr_dev;     /* nullable: the learning rate on the device, instead of lr */
   int32_t n_tensors;
-  int32_t dtype;           /* of params */
-  int32_t grad_dtype;
+  int32_t dtype;           /* of params and gradients */
   int32_t state_bits;
+  int32_t reserved;
 } SdehAdamwGroup;
 typedef struct {
   double max_norm;         /* 0 = no clipping; the norm is that of the gradients of all groups */

@@ -2,7 +2,7 @@
 //
 // Bounded by memory: fp32 with 32-bit moments reads and writes 28 bytes an entry (and the gradient's 4 once more for the norm), bf16 with 8-bit
 // moments 10 (and 2).  Two launches, however many tensors: the first forms partial sums of the gradients' squares and the tensors' coefficients
-// (step counters, bias corrections), the second adds the partial sums up again in every workgroup -- 512 doubles from L2 -- and updates.  The
+// (step counters, bias corrections), the second adds the partial sums up again in every workgroup -- 2048 doubles from L2 -- and updates.  The
 // tensors' pointers travel as kernel arguments, 48 tensors a launch: no table on the device, nothing to keep or to invalidate.
 #include "sdeh_elem.hpp"
 
@@ -11,11 +11,11 @@ namespace sdeh {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTensors = 48;       // of one launch: 48 x 64 bytes of arguments (4 KB are certain)
-constexpr int kNormBlocks = 512;   // partial sums of a step, over all its launches
+constexpr int kTensors = 48;       // of one launch: 48 x 72 bytes of arguments (4 KB are certain)
+constexpr int kNormBlocks = 2048;  // partial sums of a step, over all its launches
 constexpr int kBlock = SDEH_MOMENT_BLOCK;
-constexpr int kChunk = 4096;       // entries of a unit of work: 16 blocks of 8-bit moments
-static_assert(kChunk % kBlock == 0 && kBlock == 256, "a wave holds a block of moments, four entries a lane");
+constexpr long long kCacheBytes = 256ll << 20;
+static_assert(kBlock == 256, "a wave holds a block of moments, four entries a lane");
 
 struct Tensor {
   void* p;
@@ -24,6 +24,7 @@ struct Tensor {
   void* v;
   uint8_t* m_top;
   uint8_t* v_top;
+  float* step;
   long long n;
   unsigned first_block;
   unsigned chunk_end;  // units of work up to and including this tensor
@@ -31,13 +32,22 @@ struct Tensor {
 
 struct Batch {
   Tensor t[kTensors];
-  int n, first;       // tensors here; the first one's place among all
-  unsigned chunks;
+  int n, first;     // tensors here; the first one's place among all
+  unsigned chunks;  // units of work: `chunk` entries of one tensor, a multiple of four blocks of moments
+  int chunk;
 };
 
 struct Coef {
   float step_size, inv_root, decay;  // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), 1 - lr weight_decay
   unsigned key;                      // of the rounding bits: seed and t
+};
+
+struct Hyper {
+  double lr, beta1, beta2, weight_decay;
+  const float* lr_dev;
+  const uint8_t* ok;
+  unsigned seed;
+  Coef* coef;
 };
 
 struct Common {
@@ -62,60 +72,59 @@ __device__ __forceinline__ int find_tensor(const Batch& b, unsigned chunk) {
   return lo;
 }
 
-struct BeginArgs {
-  float* step[kTensors];
-  int n, first;
-  double lr, beta1, beta2, weight_decay;
-  const float* lr_dev;
-  const uint8_t* ok;
-  unsigned seed;
-  Coef* coef;
-};
-
 // step counters and what follows from them, one thread a tensor
-__global__ __launch_bounds__(64) void adamw_begin_kernel(BeginArgs a) {
+__device__ __forceinline__ void begin_step(const Batch& b, const Hyper& h) {
   const int i = threadIdx.x;
-  if (i >= a.n || (a.ok != nullptr && *a.ok == 0)) return;
-  const float t = *a.step[i] + 1.0f;
-  *a.step[i] = t;
-  const double lr = a.lr_dev != nullptr ? (double)*a.lr_dev : a.lr;
+  if (i >= b.n || (h.ok != nullptr && *h.ok == 0)) return;
+  const float t = *b.t[i].step + 1.0f;
+  *b.t[i].step = t;
+  const double lr = h.lr_dev != nullptr ? (double)*h.lr_dev : h.lr;
   Coef c;
-  c.step_size = (float)(lr / (1.0 - pow(a.beta1, (double)t)));
-  c.inv_root = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
-  c.decay = (float)(1.0 - lr * a.weight_decay);
-  c.key = a.seed * 0x3C6EF373u + (unsigned)t * 0xBB67AE85u;
-  a.coef[a.first + i] = c;
+  c.step_size = (float)(lr / (1.0 - pow(h.beta1, (double)t)));
+  c.inv_root = (float)(1.0 / sqrt(1.0 - pow(h.beta2, (double)t)));
+  c.decay = (float)(1.0 - lr * h.weight_decay);
+  c.key = h.seed * 0x3C6EF373u + (unsigned)t * 0xBB67AE85u;
+  h.coef[b.first + i] = c;
 }
 
+__global__ __launch_bounds__(64) void adamw_begin_kernel(Batch b, Hyper h) { begin_step(b, h); }
+
+// partial sums of the gradients' squares, by workgroups 1 ..; workgroup 0 begins the step
 template <typename G>
-__global__ __launch_bounds__(kThreads) void adamw_norm_kernel(Batch b, double* part) {
+__global__ __launch_bounds__(kThreads) void adamw_norm_kernel(Batch b, Hyper h, double* part) {
+  if (blockIdx.x == 0) {
+    begin_step(b, h);
+    return;
+  }
+  constexpr int V = 16 / (int)sizeof(G);
   double s = 0.0;
-  for (unsigned chunk = blockIdx.x; chunk < b.chunks; chunk += gridDim.x) {
+  for (unsigned chunk = blockIdx.x - 1; chunk < b.chunks; chunk += gridDim.x - 1) {
     const int k = find_tensor(b, chunk);
     const unsigned first = k > 0 ? b.t[k - 1].chunk_end : 0u;
-    const long long at = (long long)(chunk - first) * kChunk;
-    const int n = (int)(b.t[k].n - at < kChunk ? b.t[k].n - at : kChunk);
+    const long long at = (long long)(chunk - first) * b.chunk;
+    const int n = (int)(b.t[k].n - at < b.chunk ? b.t[k].n - at : b.chunk);
     const G* g = static_cast<const G*>(b.t[k].g) + at;
-    if (n == kChunk && (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(G) - 1)) == 0) {
+    if ((reinterpret_cast<uintptr_t>(g) & 15) == 0) {
+      const int body = n / V * V;
+#pragma unroll 4
+      for (int j = V * threadIdx.x; j < body; j += V * kThreads) {
+        float x[V];
+        unpack<G, V>(load_raw(g + j), x);
 #pragma unroll
-      for (int j = 0; j < kChunk; j += 4 * kThreads) {
-        float x[4];
-        load_pack<G, 4>(g + j + 4 * threadIdx.x, x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s = fma((double)x[e], (double)x[e], s);
+        for (int e = 0; e < V; ++e) s = fma((double)x[e], (double)x[e], s);
       }
+      for (int j = body + threadIdx.x; j < n; j += kThreads) s = fma((double)(float)g[j], (double)(float)g[j], s);
     } else {
       for (int j = threadIdx.x; j < n; j += kThreads) s = fma((double)(float)g[j], (double)(float)g[j], s);
     }
   }
   s = block_sum<kThreads>(s);
-  if (threadIdx.x == 0) part[blockIdx.x] = s;
+  if (threadIdx.x == 0) part[blockIdx.x - 1] = s;
 }
 
 // 32 bits that are a function of key and place: an odd multiple of the place, mixed by two rounds of shift, xor and multiplication (constants: 2^32 over
 // the golden ratio, and binary digits of the square roots of 2 and 3)
-__device__ __forceinline__ unsigned rounding_bits(unsigned key, unsigned place) {
-  unsigned x = place * 0x9E3779B1u + key;
+__device__ __forceinline__ unsigned rounding_bits(unsigned x) {  // x = place * 0x9E3779B1 + key
   x ^= x >> 16;
   x *= 0x6A09E667u;
   x ^= x >> 15;
@@ -141,32 +150,212 @@ __device__ __forceinline__ float product(float x, float y) {
   return x * y;
 }
 
+// The hardware's square root and reciprocal (one unit in the last place each) are enough for an update that is lr times smaller than what it is added to;
+// its square root takes no subnormal numbers: those are scaled.
 __device__ __forceinline__ float new_param(float p, float m, float v, const Coef& c, float eps) {
-  const float denom = fmaf(sqrtf(v), c.inv_root, eps);
-  return fmaf(p, c.decay, -c.step_size * (m / denom));
+  const bool low = v < 0x1p-96f;
+  const float root = __builtin_amdgcn_sqrtf(low ? v * 0x1p64f : v) * (low ? 0x1p-32f : 1.0f);
+  return fmaf(p, c.decay, -c.step_size * (m * __builtin_amdgcn_rcpf(fmaf(root, c.inv_root, eps))));
 }
 
-// One entry block of 8-bit moments per wave: lane l holds entries 4 l .. 4 l + 3 (x, n_live of them).  Returns the four codes and the block's top.
+// the largest value of a wave, in a scalar register (shifts within rows of 16 lanes, then rows to rows; 0 comes in from outside)
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+#define SDEH_MAX_STEP(ctrl)                                                                                   \
+  {                                                                                                           \
+    const unsigned y = (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true);                \
+    x = y > x ? y : x;                                                                                        \
+  }
+  SDEH_MAX_STEP(0x111)  // row_shr:1
+  SDEH_MAX_STEP(0x112)
+  SDEH_MAX_STEP(0x114)
+  SDEH_MAX_STEP(0x118)
+  SDEH_MAX_STEP(0x142)  // row_bcast:15
+  SDEH_MAX_STEP(0x143)  // row_bcast:31
+#undef SDEH_MAX_STEP
+  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+__device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+// Codes of four moments from q = (bits + random) >> 20: eight bits of exponent, three of mantissa, rounded.
 template <bool SIGNED>
 __device__ __forceinline__ unsigned to_codes(const unsigned (&q)[4], const float (&x)[4], int top) {
-  const int depth = SIGNED ? 15 : 31, base = 8 * (top - depth);
+  const int base = 8 * (top - (SIGNED ? 15 : 31));
   unsigned out = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    int c = (int)q[e] - base;
     const unsigned bits = __float_as_uint(x[e]);
-    if (SIGNED) {
-      c = c < 1 ? 0 : c > 127 ? 127 : c;  // (above: a NaN whose payload is all ones)
-      c |= (bits >> 24) & 128u;
-    } else {
-      c = (bits & 0x7FFFFFFFu) == 0u ? 0 : c < 1 ? 1 : c > 255 ? 255 : c;  // (a second moment above 0 stays above 0: it divides)
-    }
-    out |= (unsigned)c << (8 * e);
+    unsigned c;
+    if (SIGNED)
+      c = (unsigned)clamp_int((int)q[e] - base, 0, 127) | (bits >> 24 & 128u);  // (127 cuts a NaN whose payload is all ones)
+    else
+      c = (bits & 0x7FFFFFFFu) == 0u ? 0u : (unsigned)clamp_int((int)q[e] - base, 1, 255);  // (a second moment above 0 stays above 0: it divides)
+    out |= c << (8 * e);
   }
   return out;
 }
 
-template <typename P, typename G, int BITS>
+// Four neighbouring entries of a lane, a block of 256 of a wave.  STREAM: past the caches (sdeh_elem.hpp).
+template <typename T, bool STREAM>
+__device__ __forceinline__ void get(const T* __restrict__ p, float (&x)[4]) {
+  if constexpr (STREAM)
+    stream_in<T, 4>(p, x);
+  else
+    load_pack<T, 4>(p, x);
+}
+template <typename T, bool STREAM>
+__device__ __forceinline__ void put(T* __restrict__ p, const float (&x)[4]) {
+  if constexpr (STREAM)
+    stream_out<T, 4>(p, x);
+  else
+    store_pack<T, 4>(p, x);
+}
+template <bool STREAM>
+__device__ __forceinline__ unsigned get_codes(const uint8_t* p) {
+  const unsigned* q = reinterpret_cast<const unsigned*>(p);
+  return STREAM ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool STREAM>
+__device__ __forceinline__ void put_codes(uint8_t* p, unsigned c) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(c, reinterpret_cast<unsigned*>(p));
+  else
+    *reinterpret_cast<unsigned*>(p) = c;
+}
+
+template <typename P, int BITS, bool STREAM>
+struct Four {
+  float p[4], g[4], m[4], v[4];
+  unsigned cm, cv, tm, tv;
+
+  // `live` of the four exist; FAST: all of them, and aligned
+  template <bool FAST>
+  __device__ __forceinline__ void load(const Tensor& t, long long i, int live) {
+    const P* tp = static_cast<const P*>(t.p) + i;
+    const P* tg = static_cast<const P*>(t.g) + i;
+    if (FAST) {
+      get<P, STREAM>(tp, p);
+      load_pack<P, 4>(tg, g);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[e] = e < live ? (float)tp[e] : 0.0f;
+        g[e] = e < live ? (float)tg[e] : 0.0f;
+      }
+    }
+    if constexpr (BITS == 8) {
+      const uint8_t* m8 = static_cast<const uint8_t*>(t.m) + i;
+      const uint8_t* v8 = static_cast<const uint8_t*>(t.v) + i;
+      if (FAST) {
+        cm = get_codes<STREAM>(m8);
+        cv = get_codes<STREAM>(v8);
+      } else {
+        cm = cv = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (e < live) {
+            cm |= (unsigned)m8[e] << (8 * e);
+            cv |= (unsigned)v8[e] << (8 * e);
+          }
+        }
+      }
+      tm = t.m_top[i >> 8];  // (i - 4 lane is a multiple of 256, and i >> 8 the block, in every lane)
+      tv = t.v_top[i >> 8];
+    } else {
+      const float* fm = static_cast<const float*>(t.m) + i;
+      const float* fv = static_cast<const float*>(t.v) + i;
+      if (FAST) {
+        get<float, STREAM>(fm, m);
+        get<float, STREAM>(fv, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          m[e] = e < live ? fm[e] : 0.0f;
+          v[e] = e < live ? fv[e] : 0.0f;
+        }
+      }
+    }
+  }
+
+  template <bool FAST>
+  __device__ __forceinline__ void update(const Tensor& t, const Common& a, const Coef& c, float scale, long long i, int live) {
+    if constexpr (BITS == 8) {
+      const int bm = 8 * ((int)tm - 15), bv = 8 * ((int)tv - 31);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        m[e] = from_code<true>(cm >> (8 * e) & 255u, bm);
+        v[e] = from_code<false>(cv >> (8 * e) & 255u, bv);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y = product(g[e], scale);  // (scale is 1 without clipping: exact)
+      m[e] = blend(a.beta1, m[e], a.rest1, y);
+      v[e] = blend(a.beta2, v[e], a.rest2, product(y, y));
+      p[e] = new_param(p[e], m[e], v[e], c, a.eps);
+    }
+    P* tp = static_cast<P*>(t.p) + i;
+    if (FAST) {
+      put<P, STREAM>(tp, p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < live) tp[e] = static_cast<P>(p[e]);
+    }
+    if constexpr (BITS == 8) {
+      unsigned qm[4], qv[4], most_m = 0, most_v = 0;
+      const unsigned x = ((t.first_block << 8) + (unsigned)i) * 0x9E3779B1u + c.key;  // (place modulo 2^32)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned r = rounding_bits(x + e * 0x9E3779B1u);
+        qm[e] = ((__float_as_uint(m[e]) & 0x7FFFFFFFu) + ((r << 4 & 0xFFFF0u) | 8u)) >> 20;
+        qv[e] = ((__float_as_uint(v[e]) & 0x7FFFFFFFu) + ((r >> 12 & 0xFFFF0u) | 8u)) >> 20;
+        if (FAST || e < live) {
+          most_m = qm[e] > most_m ? qm[e] : most_m;
+          most_v = qv[e] > most_v ? qv[e] : most_v;
+        }
+      }
+      const int top_m = clamp_int((int)(wave_max(most_m) >> 3), 16, 255), top_v = clamp_int((int)(wave_max(most_v) >> 3), 32, 255);
+      cm = to_codes<true>(qm, m, top_m);
+      cv = to_codes<false>(qv, v, top_v);
+      uint8_t* m8 = static_cast<uint8_t*>(t.m) + i;
+      uint8_t* v8 = static_cast<uint8_t*>(t.v) + i;
+      if (FAST) {
+        put_codes<STREAM>(m8, cm);
+        put_codes<STREAM>(v8, cv);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (e < live) {
+            m8[e] = (uint8_t)(cm >> (8 * e));
+            v8[e] = (uint8_t)(cv >> (8 * e));
+          }
+        }
+      }
+      if ((threadIdx.x & 63) == 0) {
+        t.m_top[i >> 8] = (uint8_t)top_m;
+        t.v_top[i >> 8] = (uint8_t)top_v;
+      }
+    } else {
+      float* fm = static_cast<float*>(t.m) + i;
+      float* fv = static_cast<float*>(t.v) + i;
+      if (FAST) {
+        put<float, STREAM>(fm, m);
+        put<float, STREAM>(fv, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (e < live) {
+            fm[e] = m[e];
+            fv[e] = v[e];
+          }
+        }
+      }
+    }
+  }
+};
+
+template <typename P, int BITS, bool STREAM>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(Batch b, Common a) {
   if (a.ok != nullptr && *a.ok == 0) return;
   float scale = 1.0f;
@@ -179,140 +368,39 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(Batch b, Common a) {
     if (a.norm != nullptr && b.first == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = (float)norm;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (unsigned chunk = blockIdx.x; chunk < b.chunks; chunk += gridDim.x) {
+  // (from the last entries to the first: the gradients that the norm read last may still be in the cache)
+  for (unsigned turn = blockIdx.x; turn < b.chunks; turn += gridDim.x) {
+    const unsigned chunk = b.chunks - 1 - turn;
     const int k = find_tensor(b, chunk);
     const Tensor& t = b.t[k];
     const unsigned first = k > 0 ? b.t[k - 1].chunk_end : 0u;
     const Coef coef = a.coef[b.first + k];
-    const long long at = (long long)(chunk - first) * kChunk;
-    P* p = static_cast<P*>(t.p) + at;
-    const G* g = static_cast<const G*>(t.g) + at;
-    const int n = (int)(t.n - at < kChunk ? t.n - at : kChunk);
-    const bool wide = (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(P) - 1)) == 0 && (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(G) - 1)) == 0 &&
-                      (reinterpret_cast<uintptr_t>(t.m) & 15) == 0 && (reinterpret_cast<uintptr_t>(t.v) & 15) == 0;
-    for (int j = kBlock * wave; j < n; j += kBlock * (kThreads / 64)) {
-      const int i = j + 4 * lane, live = n - i < 0 ? 0 : n - i < 4 ? n - i : 4;
-      const bool fast = wide && live == 4;
-      float xp[4] = {0.f, 0.f, 0.f, 0.f}, xg[4] = {0.f, 0.f, 0.f, 0.f}, xm[4] = {0.f, 0.f, 0.f, 0.f}, xv[4] = {0.f, 0.f, 0.f, 0.f};
-      if (fast) {
-        load_pack<P, 4>(p + i, xp);
-        load_pack<G, 4>(g + i, xg);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < live) {
-            xp[e] = (float)p[i + e];
-            xg[e] = (float)g[i + e];
-          }
+    const long long at = (long long)(chunk - first) * b.chunk;
+    const long long end = t.n - at < b.chunk ? t.n : at + b.chunk;
+    const bool wide = (reinterpret_cast<uintptr_t>(t.p) & (4 * sizeof(P) - 1)) == 0 && (reinterpret_cast<uintptr_t>(t.g) & (4 * sizeof(P) - 1)) == 0 &&
+                      ((reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) & (BITS == 8 ? 3 : 15)) == 0;
+    long long j = at + kBlock * wave;
+    if (wide) {
+      // two blocks at a time: both blocks' loads are on their way before the first is computed
+      for (; j + kThreads * 4 + kBlock <= end; j += 2 * kThreads * 4) {
+        Four<P, BITS, STREAM> x, y;
+        const long long i = j + 4 * lane;
+        x.template load<true>(t, i, 4);
+        y.template load<true>(t, i + kThreads * 4, 4);
+        x.template update<true>(t, a, coef, scale, i, 4);
+        y.template update<true>(t, a, coef, scale, i + kThreads * 4, 4);
       }
-      const long long block = (at + j) / kBlock;
-      if constexpr (BITS == 8) {
-        const uint8_t* cm = static_cast<const uint8_t*>(t.m) + at + i;
-        const uint8_t* cv = static_cast<const uint8_t*>(t.v) + at + i;
-        unsigned km = 0, kv = 0;
-        if (fast) {
-          km = *reinterpret_cast<const unsigned*>(cm);
-          kv = *reinterpret_cast<const unsigned*>(cv);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e < live) {
-              km |= (unsigned)cm[e] << (8 * e);
-              kv |= (unsigned)cv[e] << (8 * e);
-            }
-        }
-        const int bm = 8 * ((int)t.m_top[block] - 15), bv = 8 * ((int)t.v_top[block] - 31);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          xm[e] = from_code<true>(km >> (8 * e) & 255u, bm);
-          xv[e] = from_code<false>(kv >> (8 * e) & 255u, bv);
-        }
+    }
+    for (; j < end; j += kThreads * 4) {
+      Four<P, BITS, STREAM> x;
+      const long long i = j + 4 * lane;
+      if (wide && j + kBlock <= end) {
+        x.template load<true>(t, i, 4);
+        x.template update<true>(t, a, coef, scale, i, 4);
       } else {
-        const float* fm = static_cast<const float*>(t.m) + at + i;
-        const float* fv = static_cast<const float*>(t.v) + at + i;
-        if (fast) {
-          load_pack<float, 4>(fm, xm);
-          load_pack<float, 4>(fv, xv);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e < live) {
-              xm[e] = fm[e];
-              xv[e] = fv[e];
-            }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float y = a.max_norm > 0.0 ? product(xg[e], scale) : xg[e];
-        xm[e] = blend(a.beta1, xm[e], a.rest1, y);
-        xv[e] = blend(a.beta2, xv[e], a.rest2, product(y, y));
-        xp[e] = new_param(xp[e], xm[e], xv[e], coef, a.eps);
-      }
-      if (fast) {
-        store_pack<P, 4>(p + i, xp);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < live) p[i + e] = static_cast<P>(xp[e]);
-      }
-      if constexpr (BITS == 8) {
-        unsigned qm[4], qv[4], most_m = 0, most_v = 0;
-        const unsigned place = (t.first_block + (unsigned)block) * (unsigned)kBlock + 4u * lane;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned r = rounding_bits(coef.key, place + e);
-          qm[e] = ((__float_as_uint(xm[e]) & 0x7FFFFFFFu) + ((r & 0xFFFFu) << 4) + 8u) >> 20;
-          qv[e] = ((__float_as_uint(xv[e]) & 0x7FFFFFFFu) + ((r >> 16) << 4) + 8u) >> 20;
-          if (e < live) {
-            most_m = qm[e] > most_m ? qm[e] : most_m;
-            most_v = qv[e] > most_v ? qv[e] : most_v;
-          }
-        }
-        // (both maxima in one word: 16 bits hold eight bits of exponent)
-        unsigned most = (most_m >> 3) << 16 | (most_v >> 3);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-          const unsigned other = __shfl_xor(most, o, 64);
-          const unsigned h = other >> 16 > most >> 16 ? other & 0xFFFF0000u : most & 0xFFFF0000u;
-          const unsigned l = (other & 0xFFFFu) > (most & 0xFFFFu) ? other & 0xFFFFu : most & 0xFFFFu;
-          most = h | l;
-        }
-        int top_m = (int)(most >> 16), top_v = (int)(most & 0xFFFFu);
-        top_m = top_m < 16 ? 16 : top_m > 255 ? 255 : top_m;
-        top_v = top_v < 32 ? 32 : top_v > 255 ? 255 : top_v;
-        const unsigned km = to_codes<true>(qm, xm, top_m), kv = to_codes<false>(qv, xv, top_v);
-        uint8_t* cm = static_cast<uint8_t*>(t.m) + at + i;
-        uint8_t* cv = static_cast<uint8_t*>(t.v) + at + i;
-        if (fast) {
-          *reinterpret_cast<unsigned*>(cm) = km;
-          *reinterpret_cast<unsigned*>(cv) = kv;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e < live) {
-              cm[e] = (uint8_t)(km >> (8 * e));
-              cv[e] = (uint8_t)(kv >> (8 * e));
-            }
-        }
-        if (lane == 0) {
-          t.m_top[block] = (uint8_t)top_m;
-          t.v_top[block] = (uint8_t)top_v;
-        }
-      } else {
-        float* fm = static_cast<float*>(t.m) + at + i;
-        float* fv = static_cast<float*>(t.v) + at + i;
-        if (fast) {
-          store_pack<float, 4>(fm, xm);
-          store_pack<float, 4>(fv, xv);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e < live) {
-              fm[e] = xm[e];
-              fv[e] = xv[e];
-            }
-        }
+        const int live = end - i < 0 ? 0 : end - i < 4 ? (int)(end - i) : 4;
+        x.template load<false>(t, i, live);
+        x.template update<false>(t, a, coef, scale, i, live);
       }
     }
   }
@@ -336,22 +424,20 @@ __global__ __launch_bounds__(kThreads) void adamw_moments_kernel(const uint8_t* 
   }
 }
 
-template <typename P, typename G>
-void launch_update(const Batch& b, const Common& c, int bits, unsigned grid, hipStream_t stream) {
-  if (bits == 8)
-    hipLaunchKernelGGL((adamw_kernel<P, G, 8>), dim3(grid), dim3(kThreads), 0, stream, b, c);
+template <typename P, int BITS>
+void launch_update_b(const Batch& b, const Common& c, bool past_caches, unsigned grid, hipStream_t stream) {
+  if (past_caches)
+    hipLaunchKernelGGL((adamw_kernel<P, BITS, true>), dim3(grid), dim3(kThreads), 0, stream, b, c);
   else
-    hipLaunchKernelGGL((adamw_kernel<P, G, 32>), dim3(grid), dim3(kThreads), 0, stream, b, c);
+    hipLaunchKernelGGL((adamw_kernel<P, BITS, false>), dim3(grid), dim3(kThreads), 0, stream, b, c);
 }
 
 template <typename P>
-void launch_update_g(const Batch& b, const Common& c, int grad_dtype, int bits, unsigned grid, hipStream_t stream) {
-  if (grad_dtype == SDEH_F32)
-    launch_update<P, float>(b, c, bits, grid, stream);
-  else if (grad_dtype == SDEH_BF16)
-    launch_update<P, bf16_t>(b, c, bits, grid, stream);
+void launch_update(const Batch& b, const Common& c, int bits, bool past_caches, unsigned grid, hipStream_t stream) {
+  if (bits == 8)
+    launch_update_b<P, 8>(b, c, past_caches, grid, stream);
   else
-    launch_update<P, f16_t>(b, c, bits, grid, stream);
+    launch_update_b<P, 32>(b, c, past_caches, grid, stream);
 }
 
 }  // namespace
@@ -363,8 +449,20 @@ int launch_adamw_step(const SdehAdamw& p, const SdehAdamwGroup* groups, const Sd
   double* part = reinterpret_cast<double*>(scratch);
   Coef* coef = reinterpret_cast<Coef*>(scratch + kNormBlocks * 2ll);
   int batches = 0, n_part = 0;
-  for (int k = 0; k < p.n_groups; ++k) batches += (groups[k].n_tensors + kTensors - 1) / kTensors;
+  long long entries = 0, bytes = 0;
+  for (int k = 0, at = 0; k < p.n_groups; ++k) {
+    batches += (groups[k].n_tensors + kTensors - 1) / kTensors;
+    const int each = (groups[k].dtype == SDEH_F32 ? 8 : 4) + groups[k].state_bits / 4;
+    for (const int end = at + groups[k].n_tensors; at < end; ++at) {
+      entries += tensors[at].numel;
+      bytes += tensors[at].numel * each;
+    }
+  }
   if (batches > kNormBlocks) return SDEH_ERR_UNSUPPORTED;
+  // small units while there are not enough of them to go round
+  const int chunk = entries <= 2048ll * 1024 ? 1024 : 8192;
+  // what does not fit the 256 MB cache anyway goes past it and leaves it to the gradients, which are read twice
+  const bool past_caches = bytes > kCacheBytes;
   // pass 0: refuse what does not fit, before anything runs; pass 1: coefficients and norm; pass 2: update
   for (int pass = 0; pass < 3; ++pass) {
     int first = 0, left = batches;
@@ -377,35 +475,27 @@ int launch_adamw_step(const SdehAdamw& p, const SdehAdamwGroup* groups, const Sd
         long long chunks = 0;
         for (int i = 0; i < b.n; ++i) {
           const SdehAdamwTensor& t = tensors[b.first + i];
-          chunks += (t.numel + kChunk - 1) / kChunk;
+          chunks += (t.numel + chunk - 1) / chunk;
           if (chunks > 0x7FFFFFFFll || t.first_block + (t.numel + kBlock - 1) / kBlock > 0xFFFFFFFFll) return SDEH_ERR_UNSUPPORTED;
-          b.t[i] = Tensor{t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_top, t.exp_avg_sq_top, t.numel, (unsigned)t.first_block, (unsigned)chunks};
+          b.t[i] = Tensor{t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_top, t.exp_avg_sq_top, t.step, t.numel,
+                          (unsigned)t.first_block, (unsigned)chunks};
         }
         b.chunks = (unsigned)chunks;
+        b.chunk = chunk;
         if (pass == 1) {
-          BeginArgs begin{};
-          for (int i = 0; i < b.n; ++i) begin.step[i] = tensors[b.first + i].step;
-          begin.n = b.n;
-          begin.first = b.first;
-          begin.lr = g.lr;
-          begin.beta1 = g.beta1;
-          begin.beta2 = g.beta2;
-          begin.weight_decay = g.weight_decay;
-          begin.lr_dev = g.lr_dev;
-          begin.ok = p.ok;
-          begin.seed = p.seed;
-          begin.coef = coef;
-          hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(64), 0, stream, begin);
+          const Hyper h{g.lr, g.beta1, g.beta2, g.weight_decay, g.lr_dev, p.ok, p.seed, coef};
           if (p.max_norm > 0.0 && chunks > 0) {
             const long long room = (kNormBlocks - n_part) / left;  // (each batch its share of the partial sums)
             const unsigned grid = (unsigned)(chunks < room ? chunks : room);
-            if (g.grad_dtype == SDEH_F32)
-              hipLaunchKernelGGL(adamw_norm_kernel<float>, dim3(grid), dim3(kThreads), 0, stream, b, part + n_part);
-            else if (g.grad_dtype == SDEH_BF16)
-              hipLaunchKernelGGL(adamw_norm_kernel<bf16_t>, dim3(grid), dim3(kThreads), 0, stream, b, part + n_part);
+            if (g.dtype == SDEH_F32)
+              hipLaunchKernelGGL(adamw_norm_kernel<float>, dim3(grid + 1), dim3(kThreads), 0, stream, b, h, part + n_part);
+            else if (g.dtype == SDEH_BF16)
+              hipLaunchKernelGGL(adamw_norm_kernel<bf16_t>, dim3(grid + 1), dim3(kThreads), 0, stream, b, h, part + n_part);
             else
-              hipLaunchKernelGGL(adamw_norm_kernel<f16_t>, dim3(grid), dim3(kThreads), 0, stream, b, part + n_part);
+              hipLaunchKernelGGL(adamw_norm_kernel<f16_t>, dim3(grid + 1), dim3(kThreads), 0, stream, b, h, part + n_part);
             n_part += (int)grid;
+          } else {
+            hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(64), 0, stream, b, h);
           }
         } else if (pass == 2) {
           Common c{};
@@ -422,11 +512,11 @@ int launch_adamw_step(const SdehAdamw& p, const SdehAdamwGroup* groups, const Sd
           c.norm = p.norm;
           const unsigned grid = (unsigned)(chunks < 2048 ? (chunks > 0 ? chunks : 1) : 2048);
           if (g.dtype == SDEH_F32)
-            launch_update_g<float>(b, c, g.grad_dtype, g.state_bits, grid, stream);
+            launch_update<float>(b, c, g.state_bits, past_caches, grid, stream);
           else if (g.dtype == SDEH_BF16)
-            launch_update_g<bf16_t>(b, c, g.grad_dtype, g.state_bits, grid, stream);
+            launch_update<bf16_t>(b, c, g.state_bits, past_caches, grid, stream);
           else
-            launch_update_g<f16_t>(b, c, g.grad_dtype, g.state_bits, grid, stream);
+            launch_update<f16_t>(b, c, g.state_bits, past_caches, grid, stream);
         }
       }
       first += g.n_tensors;

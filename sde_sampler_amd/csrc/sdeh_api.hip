@@ -2066,7 +2066,7 @@ int32_t sdeh_adamw_step(const SdehAdamw* p, const SdehAdamwGroup* groups, const 
   int64_t at = 0;
   for (int32_t k = 0; k < p->n_groups; ++k) {
     const SdehAdamwGroup& g = groups[k];
-    if (!dtype_ok(g.dtype) || !dtype_ok(g.grad_dtype) || (g.state_bits != 8 && g.state_bits != 32))
+    if (!dtype_ok(g.dtype) || (g.state_bits != 8 && g.state_bits != 32))
       return fail(SDEH_ERR_INVALID, "adamw_step: unknown type, or moments in neither 8 nor 32 bits");
     if (!(g.beta1 >= 0.0 && g.beta1 < 1.0) || !(g.beta2 >= 0.0 && g.beta2 < 1.0) || !(g.eps >= 0.0) || !(g.lr >= 0.0) || !(g.weight_decay >= 0.0))
       return fail(SDEH_ERR_INVALID, "adamw_step: lr, eps and weight_decay are >= 0, betas in [0, 1)");

@@ -45,6 +45,33 @@ __device__ __forceinline__ void unpack(const Raw& r, float (&x)[V]) {
   for (int i = 0; i < V; ++i) x[i] = static_cast<float>(k.v[i]);
 }
 
+// the same past the caches, for tensors that are read and written once a pass and do not fit them
+template <int B>
+struct Bits;
+template <>
+struct Bits<16> {
+  typedef Raw type;
+};
+template <>
+struct Bits<8> {
+  typedef unsigned type __attribute__((ext_vector_type(2)));
+};
+template <typename T, int V>
+__device__ __forceinline__ void stream_in(const T* __restrict__ p, float (&x)[V]) {
+  typedef typename Bits<V * sizeof(T)>::type B;
+  const Pack<T, V> k = __builtin_bit_cast(Pack<T, V>, __builtin_nontemporal_load(reinterpret_cast<const B*>(p)));
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = static_cast<float>(k.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void stream_out(T* __restrict__ p, const float (&x)[V]) {
+  typedef typename Bits<V * sizeof(T)>::type B;
+  Pack<T, V> k;
+#pragma unroll
+  for (int i = 0; i < V; ++i) k.v[i] = static_cast<T>(x[i]);
+  __builtin_nontemporal_store(__builtin_bit_cast(B, k), reinterpret_cast<B*>(p));
+}
+
 // one element of a tensor whose type is known at run time
 __device__ __forceinline__ float load_as(const void* p, int dtype, long long i) {
   if (dtype == SDEH_F32) return static_cast<const float*>(p)[i];

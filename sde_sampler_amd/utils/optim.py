@@ -223,7 +223,7 @@ class AdamW(torch.optim.Optimizer):
             for b in buckets:
                 rows, held = b.rows()
                 if len(rows):
-                    groups.append(L.ADAMW_GROUP.pack(lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, len(rows), b.code, b.code, b.bits))
+                    groups.append(L.ADAMW_GROUP.pack(lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, len(rows), b.code, b.bits, 0))
                     tables.append(rows)
                     keep.append(held)
         if not groups:

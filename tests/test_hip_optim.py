@@ -507,12 +507,12 @@ def test_c_entry_refuses_bad_arguments():
     lib = L.load()
     head = lambda **k: L.ADAMW.pack(k.get("clip", 1.0), 0, 0, 1, k.get("groups", 1))  # noqa: E731
     group = lambda **k: L.ADAMW_GROUP.pack(k.get("lr", 0.1), k.get("b1", 0.9), k.get("b2", 0.99), k.get("eps", 0.0), k.get("wd", 0.0), 0, k.get("n", 1),  # noqa: E731
-                                           k.get("dtype", 0), k.get("gtype", 0), k.get("bits", 32))
+                                           k.get("dtype", 0), k.get("bits", 32), 0)
     table = lambda *row: np.array(row or (64, 64, 64, 64, 0, 0, 64, 5, 0), dtype=np.int64)  # noqa: E731
     call = lambda h, g, t=table(), s=64: lib.sdeh_adamw_step(h, g, None if t is None else t.ctypes.data, s, None)  # noqa: E731
     for bad in (dict(clip=-1.0), dict(clip=math.nan), dict(groups=-1)):
         assert call(head(**bad), group()) == -1, bad
-    for bad in (dict(lr=-1.0), dict(lr=math.nan), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0), dict(wd=-1.0), dict(n=-1), dict(dtype=3), dict(gtype=-1),
+    for bad in (dict(lr=-1.0), dict(lr=math.nan), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0), dict(wd=-1.0), dict(n=-1), dict(dtype=3), dict(dtype=-1),
                 dict(bits=16), dict(bits=8)):
         assert call(head(), group(**bad)) == -1, bad
     for row in ((0, 64, 64, 64, 0, 0, 64, 5, 0), (64, 0, 64, 64, 0, 0, 64, 5, 0), (64, 64, 64, 64, 0, 0, 0, 5, 0), (64, 64, 64, 64, 0, 0, 64, -5, 0),
