@@ -268,23 +268,30 @@ def load():
 
 def dtype_code(dtype) -> int | None:
     """SdehDtype of a torch dtype, None where the kernels have none."""
-    import torch
+    if not _DTYPES:
+        import torch
 
-    return {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}.get(dtype)
+        _DTYPES.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    return _DTYPES.get(dtype)
+
+
+_DTYPES: dict = {}
+_FUNCTIONS: dict = {}
 
 
 def call(name: str, device, *args):
     """Calls a stream-ordered entry point on torch's current stream of `device` (its last argument), whichever device is current."""
-    import torch
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(load(), name)
+    from torch import _C, cuda
 
-    fn = getattr(load(), name)
     index = device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
-        status = fn(*args, stream)
+    if _C._cuda_getDevice() == index:
+        status = fn(*args, _C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(index):
-            status = fn(*args, stream)
+        with cuda.device(index):
+            status = fn(*args, _C._cuda_getCurrentRawStream(index))
     if status != 0:
         check(status)
 

@@ -9,6 +9,18 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// i = row * steps + col; by 32-bit arithmetic where i fits it (a 64-bit division takes a hundred instructions and more)
+__device__ __forceinline__ void split_index(long long i, long long steps, long long& row, long long& col) {
+  if ((unsigned long long)i >> 32 == 0ull && (unsigned long long)steps >> 32 == 0ull) {
+    const unsigned r = (unsigned)i / (unsigned)steps;
+    row = r;
+    col = (unsigned)i - r * (unsigned)steps;
+  } else {
+    row = i / steps;
+    col = i - row * steps;
+  }
+}
+
 // -------------------------------------------------------------------------------------------------------------------------------------------
 // step log-ratio: l = sum_d e dW - dt/2 e^2, e = u - v;   gradient g (dW - dt e)
 //
@@ -109,6 +121,80 @@ __global__ __launch_bounds__(kThreads) void ratio_kernel(RatioArgs a) {
   }
 }
 
+// The forward pass for rows of at least V coordinates and aligned tensors.  A vector of V elements then meets at most two rows: its lane sums the part
+// before the row's end and the part after it, and only these two numbers go through LDS (2 words for V elements instead of V).  All loads of a stretch
+// are on their way before the first is used.
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void ratio_forward_kernel(RatioArgs a, unsigned inverse) {  // inverse = ceil(2^32 / dim)
+  constexpr int kTurns = 2, kVectors = kTurns * kThreads;  // (four turns of fp32 took 140 registers: 60 instead of 54 us for 200 x 2048 x 50)
+  __shared__ float before[kVectors], after[kVectors];
+  __shared__ float row_dt[kStretchRows + 1];
+  const long long r0 = (long long)blockIdx.x * a.rows;
+  const int nr = (int)(a.rows_total - r0 < a.rows ? a.rows_total - r0 : a.rows);
+  const int d = a.dim, n = nr * d, whole = n / V;
+  const T* u = static_cast<const T*>(a.u) + r0 * d;
+  const T* v = static_cast<const T*>(a.v != nullptr ? a.v : a.u) + r0 * d;
+  const T* dw = static_cast<const T*>(a.dw) + r0 * d;
+  Raw xu[kTurns]{}, xv[kTurns]{}, xw[kTurns]{};
+#pragma unroll
+  for (int t = 0; t < kTurns; ++t) {
+    const int i = t * kThreads + threadIdx.x;
+    if (i < whole) {
+      xu[t] = load_raw(u + i * V);
+      xv[t] = load_raw(v + i * V);
+      xw[t] = load_raw(dw + i * V);
+    }
+  }
+  const long long t0 = r0 / a.batch, b0 = r0 - t0 * a.batch;  // (uniform over the workgroup)
+  for (int r = threadIdx.x; r <= nr; r += kThreads) {
+    const long long b = b0 + r, t = b < a.batch ? t0 : t0 + b / a.batch;
+    row_dt[r] = r < nr ? 0.5f * a.dt[t] : 0.0f;
+  }
+  __syncthreads();
+  const float keep = a.v != nullptr ? 1.0f : 0.0f;
+#pragma unroll
+  for (int t = 0; t < kTurns; ++t) {
+    const int i = t * kThreads + threadIdx.x;
+    if (i < whole) {
+      const int r = (int)__umulhi((unsigned)(i * V), inverse), left = (r + 1) * d - i * V;  // (elements of this row from here on)
+      float pu[V], pv[V], pw[V];
+      unpack<T, V>(xu[t], pu);
+      unpack<T, V>(xv[t], pv);
+      unpack<T, V>(xw[t], pw);
+      float s1 = 0.0f, s2 = 0.0f, a1 = 0.0f, a2 = 0.0f;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float e = keep != 0.0f ? pu[k] - pv[k] : pu[k];
+        const bool here = k < left;
+        s1 = fmaf(here ? e : 0.0f, pw[k], s1);
+        s2 = fmaf(here ? e : 0.0f, e, s2);
+        a1 = fmaf(here ? 0.0f : e, pw[k], a1);
+        a2 = fmaf(here ? 0.0f : e, e, a2);
+      }
+      before[i] = fmaf(-row_dt[r], s2, s1);
+      after[i] = left < V ? fmaf(-row_dt[r + 1], a2, a1) : 0.0f;
+    }
+  }
+  __syncthreads();
+  const int G = a.group, lane = threadIdx.x & (G - 1);
+  for (int r = threadIdx.x / G; r < nr; r += kThreads / G) {
+    const int lo = r * d, hi = lo + d, first = (lo + V - 1) / V, last = (hi - 1) / V;  // vectors that start in the row
+    float s = lane == 0 && lo % V != 0 ? after[lo / V] : 0.0f;
+    for (int i = first + lane; i <= last; i += G) {
+      if (i < whole) {
+        s += before[i];
+      } else {  // (less than a vector at the end of the last stretch)
+        for (int k = whole * V; k < n; ++k) {
+          const float e = (float)u[k] - (keep != 0.0f ? (float)v[k] : 0.0f);
+          s += e * ((float)dw[k] - row_dt[r] * e);
+        }
+      }
+    }
+    for (int o = G >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) static_cast<float*>(a.out)[r0 + r] = s;
+  }
+}
+
 // rows longer than kStagedDim: a workgroup sums one
 template <typename T>
 __global__ __launch_bounds__(kThreads) void ratio_long_kernel(RatioArgs a) {
@@ -159,7 +245,14 @@ int launch_ratio_t(RatioArgs a, hipStream_t stream) {
   if (blocks > 0x7FFFFFFFll) return SDEH_ERR_UNSUPPORTED;
   constexpr int V = 16 / (int)sizeof(T);
   const bool wide = aligned_to(a.u, 16) && aligned_to(a.dw, 16) && (a.v == nullptr || aligned_to(a.v, 16)) && (!BACK || aligned_to(a.out, 16));
-  if (wide)
+  if (wide && !BACK && a.dim >= V) {
+    a.rows = 2 * kThreads * V / a.dim / V * V;  // (whole rows, V of them: at least V as dim <= 512)
+    a.group = 1;                                // (for the vectors of a row, not its elements)
+    while (a.group < 64 && a.group * 2 * a.rows <= kThreads && a.group * 2 * V <= a.dim) a.group *= 2;
+    const long long stretches = (a.rows_total + a.rows - 1) / a.rows;
+    if (stretches > 0x7FFFFFFFll) return SDEH_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((ratio_forward_kernel<T, V>), dim3((unsigned)stretches), dim3(kThreads), 0, stream, a, (unsigned)((0x100000000ull + a.dim - 1) / a.dim));
+  } else if (wide)
     hipLaunchKernelGGL((ratio_kernel<T, V, BACK>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL((ratio_kernel<T, 1, BACK>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
@@ -402,6 +495,15 @@ __device__ __forceinline__ unsigned byte_bits(unsigned m) {
   return (t >> 7 & 1u) | (t >> 14 & 2u) | (t >> 21 & 4u) | (t >> 28 & 8u);
 }
 
+// the same of V bytes (4 or 8, aligned to as many)
+template <int V>
+__device__ __forceinline__ unsigned byte_mask(const uint8_t* m) {
+  const Pack<unsigned, V / 4> k = *reinterpret_cast<const Pack<unsigned, V / 4>*>(m);
+  unsigned ok = byte_bits(k.v[0]);
+  if constexpr (V == 8) ok |= byte_bits(k.v[1]) << 4;
+  return ok;
+}
+
 // what a pass needs throughout
 struct PolicyView {
   bool has_ref, row_weight;
@@ -454,7 +556,11 @@ __device__ __forceinline__ PolicySums policy_pass(const PolicyArgs& a) {
     const PolicyView v = policy_view(a, common_weight<NT>(a, a.n_count));
     for (long long round = 0; round < rounds; ++round) {
       const long long i = place(round) + threadIdx.x;
-      if (i < body) policy_one<T>(a, v, i / p.steps, i % p.steps, sums);
+      if (i < body) {
+        long long row, col;
+        split_index(i, p.steps, row, col);
+        policy_one<T>(a, v, row, col, sums);
+      }
     }
   } else {
     const T* lp = static_cast<const T*>(p.log_prob.data);
@@ -515,8 +621,9 @@ __device__ __forceinline__ PolicySums policy_pass(const PolicyArgs& a) {
       load_values(start_next + mine, ok_next);
       long long row = 0, col = 0;
       if constexpr (ROW) {  // (the tile's place by 64-bit arithmetic of the whole wave, the thread's in it by 32-bit arithmetic)
-        const long long r0 = start / p.steps;
-        const unsigned t = (unsigned)(start - r0 * p.steps) + (unsigned)mine, r = t / (unsigned)p.steps;
+        long long r0, c0;
+        split_index(start, p.steps, r0, c0);
+        const unsigned t = (unsigned)c0 + (unsigned)mine, r = t / (unsigned)p.steps;
         row = r0 + r;
         col = t - r * (unsigned)p.steps;
       }
@@ -734,8 +841,8 @@ struct PreferenceArgs {
   long long d_row[2], d_col[2];
 };
 
-// Sum and number of the valid entries [lo, hi) of a row, this thread's share: `me` of `team` threads.
-template <typename T, int V>
+// Sum and number of the valid entries [lo, hi) of a row, this thread's share: `me` of `team` threads, U vectors at a time.
+template <typename T, int V, int U>
 __device__ __forceinline__ void row_share(const SdehPreferenceSide& s, long long row, long long lo, long long hi, int me, int team, double& sum,
                                           long long& count) {
   const T* x = static_cast<const T*>(s.log_prob.data) + row * s.log_prob.row_stride;
@@ -748,41 +855,52 @@ __device__ __forceinline__ void row_share(const SdehPreferenceSide& s, long long
       ++count;
     }
   };
-  if (V == 1) {
+  if constexpr (V == 1) {
     for (long long i = lo + me; i < hi; i += team) one(i);
     return;
-  }
-  // contiguous planes with one row stride: entries up to the first 16-byte border (the same in every plane), vectors, the rest
-  const long long flat = row * s.log_prob.row_stride;
-  long long head = lo + (V - (flat + lo) % V) % V;
-  if (head > hi) head = hi;
-  const long long body = head + (hi - head) / V * V;
-  for (long long i = lo + me; i < head; i += team) one(i);
-  for (long long i = head + (long long)me * V; i < body; i += (long long)team * V) {
-    bool ok[V];
-    int any = 1;
-    if (m != nullptr) {
-      const Pack<uint8_t, V> k = *reinterpret_cast<const Pack<uint8_t, V>*>(m + i);
-      any = 0;
+  } else {
+    // contiguous planes with one row stride: entries up to the first 16-byte border (the same in every plane), vectors, the rest
+    const long long flat = row * s.log_prob.row_stride;
+    long long head = lo + (V - (flat + lo) % V) % V;
+    if (head > hi) head = hi;
+    const long long body = head + (hi - head) / V * V;
+    for (long long i = lo + me; i < head; i += team) one(i);
+    // the masks' loads, then the loads of those vectors that have a valid entry, then the sums
+    const T* q_at = q != nullptr ? q : x;
+    constexpr unsigned kAll = (1u << V) - 1u;
+    const long long step = (long long)team * V;
+    for (long long i = head + (long long)me * V; i < body; i += U * step) {
+      unsigned ok[U];
+      Raw a[U]{}, b[U]{};
 #pragma unroll
-      for (int j = 0; j < V; ++j) any |= ok[j] = k.v[j] != 0;
-    } else {
+      for (int t = 0; t < U; ++t) {
+        ok[t] = i + t * step < body ? kAll : 0u;
+        if (m != nullptr && ok[t] != 0u) ok[t] = byte_mask<V>(m + i + t * step);
+      }
 #pragma unroll
-      for (int j = 0; j < V; ++j) ok[j] = true;
-    }
-    if (any) {
-      float a[V], b[V];
-      load_pack<T, V>(x + i, a);
-      if (q != nullptr) load_pack<T, V>(q + i, b);
+      for (int t = 0; t < U; ++t) {
+        if (ok[t] != 0u) {
+          a[t] = load_raw(x + i + t * step);
+          b[t] = load_raw(q_at + i + t * step);
+        }
+      }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const double d = q == nullptr ? (double)a[j] : (double)a[j] - (double)b[j];
-        sum += ok[j] ? d : 0.0;
-        count += ok[j];
+      for (int t = 0; t < U; ++t) {
+        if (ok[t] != 0u) {
+          float fa[V], fb[V];
+          unpack<T, V>(a[t], fa);
+          unpack<T, V>(b[t], fb);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float at = ok[t] >> j & 1u ? fa[j] : 0.0f, bt = q != nullptr && (ok[t] >> j & 1u) ? fb[j] : 0.0f;
+            sum += (double)at - (double)bt;
+          }
+          count += __popc(ok[t]);
+        }
       }
     }
+    for (long long i = body + me; i < hi; i += team) one(i);
   }
-  for (long long i = body + me; i < hi; i += team) one(i);
 }
 
 // one workgroup a part of a row
@@ -795,7 +913,7 @@ __global__ __launch_bounds__(kThreads) void preference_sum_kernel(PreferenceArgs
   const long long lo = split * a.chunk, hi = lo + a.chunk < s.steps ? lo + a.chunk : s.steps;
   double sum = 0.0;
   long long count = 0;
-  if (lo < hi) row_share<T, V>(s, second ? line - a.p.pairs : line, lo, hi, threadIdx.x, kThreads, sum, count);
+  if (lo < hi) row_share<T, V, 4>(s, second ? line - a.p.pairs : line, lo, hi, threadIdx.x, kThreads, sum, count);
   sum = block_sum<kThreads>(sum);
   count = block_sum<kThreads>(count);
   if (threadIdx.x == 0) {
@@ -812,7 +930,7 @@ __device__ __forceinline__ void short_rows(const PreferenceArgs& a, long long fi
     const SdehPreferenceSide& s = second ? a.p.rejected : a.p.chosen;
     double sum = 0.0;
     long long count = 0;
-    row_share<T, V>(s, second ? line - a.p.pairs : line, 0, s.steps, threadIdx.x & 63, 64, sum, count);
+    row_share<T, V, 1>(s, second ? line - a.p.pairs : line, 0, s.steps, threadIdx.x & 63, 64, sum, count);
     sum = wave_sum(sum);
     count = wave_sum(count);
     if ((threadIdx.x & 63) == 0) {
@@ -908,7 +1026,8 @@ __global__ __launch_bounds__(kThreads) void preference_pair_kernel(PreferenceArg
   }
 }
 
-__global__ __launch_bounds__(kThreads) void preference_final_kernel(PreferenceArgs a) {
+// the means, from the workgroups' sums
+__device__ __forceinline__ void preference_means(const PreferenceArgs& a) {
   double loss = 0.0, correct = 0.0;
   for (int i = threadIdx.x; i < a.n_pair_blocks; i += kThreads) {
     loss += a.part[2 * i];
@@ -922,6 +1041,8 @@ __global__ __launch_bounds__(kThreads) void preference_final_kernel(PreferenceAr
   }
 }
 
+__global__ __launch_bounds__(kThreads) void preference_final_kernel(PreferenceArgs a) { preference_means(a); }
+
 // gradients of one side: the pair's slope on valid entries
 template <typename T, int V, int NT>
 __device__ __forceinline__ void spread_pass(const PreferenceArgs& a, int side, const float* slopes) {
@@ -932,32 +1053,40 @@ __device__ __forceinline__ void spread_pass(const PreferenceArgs& a, int side, c
   const long long n = a.p.pairs * s.steps, stride = (long long)gridDim.x * NT * V;
   long long i = ((long long)blockIdx.x * NT + threadIdx.x) * V;
   if (i >= n) return;
-  long long row = i / s.steps, col = i - row * s.steps;
+  long long row, col;
+  split_index(i, s.steps, row, col);
   for (; i < n; i += stride) {
-    const int live = n - i < V ? (int)(n - i) : V;
-    long long r = row, c = col;
-    float g[V], slope = slopes[r] * factor;
+    if (V > 1 && n - i >= V) {
+      float g[V];
+      if constexpr (V > 1) {
+        const unsigned ok = m == nullptr ? (1u << V) - 1u : byte_mask<V>(m + i);
+        const float slope = slopes[row] * factor;
+        if (col + V <= s.steps) {  // (one row)
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const bool ok = k < live && (m == nullptr || V > 1 || m[r * s.mask.row_stride + c * s.mask.step_stride] != 0);
-      g[k] = ok ? slope : 0.0f;
-      if (++c == s.steps && k + 1 < live) {
-        c = 0;
-        ++r;
-        slope = slopes[r] * factor;
-      }
-    }
-    if (V > 1 && live == V) {
-      if (m != nullptr) {
-        const Pack<uint8_t, V> k8 = *reinterpret_cast<const Pack<uint8_t, V>*>(m + i);
+          for (int k = 0; k < V; ++k) g[k] = ok >> k & 1u ? slope : 0.0f;
+        } else {
+          long long r = row, c = col;
 #pragma unroll
-        for (int k = 0; k < V; ++k) g[k] = k8.v[k] != 0 ? g[k] : 0.0f;
+          for (int k = 0; k < V; ++k) {
+            g[k] = ok >> k & 1u ? slopes[r] * factor : 0.0f;
+            if (++c == s.steps) {
+              c = 0;
+              r += k + 1 < V;
+            }
+          }
+        }
       }
       store_pack<T, V>(grad + i, g);
     } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (k < live) grad[i + k] = static_cast<T>(m == nullptr || V == 1 || m[i + k] != 0 ? g[k] : 0.0f);
+      long long r = row, c = col;
+      for (long long k = i; k < n && k < i + V; ++k) {
+        const bool ok = m == nullptr || m[V > 1 ? k : r * s.mask.row_stride + c * s.mask.step_stride] != 0;
+        grad[k] = static_cast<T>(ok ? slopes[r] * factor : 0.0f);
+        if (++c == s.steps) {
+          c = 0;
+          ++r;
+        }
+      }
     }
     row += a.d_row[side];
     col += a.d_col[side];
@@ -972,6 +1101,7 @@ template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void preference_grad_kernel(PreferenceArgs a) {
   const int side = blockIdx.y;
   spread_pass<T, V, kThreads>(a, side, a.slopes + side * a.p.pairs);
+  if (a.n_pair_blocks > 1 && blockIdx.x == 0 && side == 0) preference_means(a);  // (a launch less)
 }
 
 // few and short rows: everything by one workgroup
@@ -999,11 +1129,11 @@ constexpr long long kPreferenceSmall = 8192;  // entries of both sides that one 
 constexpr long long kShortRow = 1024;         // rows that a wave sums
 constexpr int kMaxSplits = 64;
 
-// parts of a row: a workgroup a part, and 1024 workgroups where rows are few
+// parts of a row: a workgroup a part of 4096 entries or more, and 3072 workgroups where rows are few (those that get padding end at once)
 int preference_splits(const SdehPreferenceLoss& p) {
   const long long longest = p.chosen.steps > p.rejected.steps ? p.chosen.steps : p.rejected.steps;
   if (longest <= kShortRow) return 1;
-  long long s = (1024 + 2 * p.pairs - 1) / (2 * p.pairs), most = (longest + 4095) / 4096;
+  long long s = (3072 + 2 * p.pairs - 1) / (2 * p.pairs), most = (longest + 4095) / 4096;
   s = s > most ? most : s;
   return (int)(s > kMaxSplits ? kMaxSplits : s < 1 ? 1 : s);
 }
@@ -1030,7 +1160,7 @@ int launch_spread_t(PreferenceArgs a, hipStream_t stream) {
   if (n == 0) return SDEH_OK;
   const int v = wide ? V : 1;
   long long blocks = (n + (long long)kThreads * v - 1) / ((long long)kThreads * v);
-  if (blocks > 1024) blocks = 1024;
+  if (blocks > 4096) blocks = 4096;
   grad_strides(a, blocks, kThreads, v);
   if (wide)
     hipLaunchKernelGGL((preference_grad_kernel<T, V>), dim3((unsigned)blocks, 2), dim3(kThreads), 0, stream, a);
@@ -1075,9 +1205,9 @@ int launch_preference_t(PreferenceArgs a, hipStream_t stream) {
   long long pair_blocks = (p.pairs + per - 1) / per;
   a.n_pair_blocks = (int)(pair_blocks > kPairBlocks ? kPairBlocks : pair_blocks);
   hipLaunchKernelGGL(preference_pair_kernel, dim3(a.n_pair_blocks), dim3(kThreads), 0, stream, a);
-  if (a.n_pair_blocks > 1) hipLaunchKernelGGL(preference_final_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+  if (a.n_pair_blocks > 1 && (a.grad[0] == nullptr || longest == 0)) hipLaunchKernelGGL(preference_final_kernel, dim3(1), dim3(kThreads), 0, stream, a);
   if (hipGetLastError() != hipSuccess) return SDEH_ERR_HIP;
-  if (a.grad[0] == nullptr) return SDEH_OK;
+  if (a.grad[0] == nullptr || longest == 0) return SDEH_OK;
   a.slopes = a.out + 2 + 2 * p.pairs;
   return launch_spread_t<T>(a, stream);
 }

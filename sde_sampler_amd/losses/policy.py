@@ -35,6 +35,20 @@ def _code(name: str, t: torch.Tensor, device=None) -> int:
     return code
 
 
+def _constant(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t.detach() if t is not None and t.requires_grad else t
+
+
+def _once(backward):
+    """`once_differentiable` where a graph of the backward pass is asked for; without one (the usual call) there is nothing to guard."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 # -- step log-ratio --------------------------------------------------------------------------------------------------------------------------
 class _StepLogRatio(torch.autograd.Function):
     @staticmethod
@@ -44,7 +58,7 @@ class _StepLogRatio(torch.autograd.Function):
         return _ratio(control, behaviour, increments, dt, code)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         control, behaviour, increments, dt = ctx.saved_tensors
         T, B, d = control.shape
@@ -82,12 +96,12 @@ def step_log_ratio(control: torch.Tensor, behaviour: torch.Tensor | None, increm
                              f"on {control.device}")
     if dt.shape != control.shape[:1] or dt.device != control.device:
         raise ValueError(f"step_log_ratio: dt must be [{control.shape[0]}] on {control.device}, got {tuple(dt.shape)} on {dt.device}")
-    control, increments = control.contiguous(), increments.detach().contiguous()
-    behaviour = None if behaviour is None else behaviour.detach().contiguous()
-    dt = dt.detach().float().contiguous()
+    control, increments = control.contiguous(), _constant(increments).contiguous()
+    behaviour = None if behaviour is None else _constant(behaviour).contiguous()
+    dt = _constant(dt).float().contiguous()
     if torch.is_grad_enabled() and control.requires_grad:
         return _StepLogRatio.apply(control, behaviour, increments, dt, code)
-    return _ratio(control.detach(), behaviour, increments, dt, code)
+    return _ratio(control, behaviour, increments, dt, code)
 
 
 # -- clipped policy loss ---------------------------------------------------------------------------------------------------------------------
@@ -105,13 +119,15 @@ def _describe_policy(log_prob, advantage, old, ref, mask, clip_low, clip_high, d
         if t is not None and (t.shape != shape or t.dtype != log_prob.dtype or t.device != dev):
             raise ValueError(f"policy_loss: {name} is {tuple(t.shape)} {t.dtype} on {t.device}, log_prob {tuple(shape)} {log_prob.dtype} on {dev}")
     adv_code = _code("policy_loss", advantage, dev)
-    if advantage.ndim == 1 and advantage.shape[0] == shape[0]:
-        advantage = advantage.unsqueeze(1)
-    elif advantage.ndim != 2:
-        raise ValueError(f"policy_loss: advantage must be [rows] or [rows, steps], got {tuple(advantage.shape)} for log_prob {tuple(shape)}")
     try:
-        if advantage.shape != shape:
-            advantage = advantage.expand(shape)
+        if advantage.ndim == 1 and advantage.shape[0] == shape[0]:
+            adv_plane = (advantage.data_ptr(), advantage.stride(0), 0)
+        elif advantage.ndim == 2:
+            if advantage.shape != shape:
+                advantage = advantage.expand(shape)
+            adv_plane = _plane(advantage)
+        else:
+            raise ValueError(f"policy_loss: advantage must be [rows] or [rows, steps], got {tuple(advantage.shape)} for log_prob {tuple(shape)}")
         if mask is not None and mask.shape != shape:
             mask = mask.expand(shape)
     except RuntimeError as exc:
@@ -122,7 +138,7 @@ def _describe_policy(log_prob, advantage, old, ref, mask, clip_low, clip_high, d
         raise ValueError(f"policy_loss: kl is one of {list(L.KL_ESTIMATORS)} and reduction one of {list(L.REDUCTIONS)}, got {kl!r} and {reduction!r}")
     if not (clip_low >= 0.0 and clip_high >= 0.0 and (dual_clip is None or dual_clip > 1.0)):
         raise ValueError(f"policy_loss: clip_low, clip_high >= 0 and dual_clip > 1, got {clip_low}, {clip_high}, {dual_clip}")
-    p = L.POLICY_LOSS.pack(*_plane(log_prob), *_plane(old), *_plane(ref), *_plane(advantage), *_plane(mask), *shape, code, adv_code,
+    p = L.POLICY_LOSS.pack(*_plane(log_prob), *_plane(old), *_plane(ref), *adv_plane, *_plane(mask), *shape, code, adv_code,
                            L.KL_ESTIMATORS[kl], L.REDUCTIONS[reduction], clip_low, clip_high, dual_clip or 0.0, kl_coef)
     return p, (log_prob, advantage, old, ref, mask)
 
@@ -148,11 +164,14 @@ class _PolicyLoss(torch.autograd.Function):
         ctx.save_for_backward(log_prob, advantage, old, ref, mask, scratch)
         ctx.packed = packed
         ctx.mark_non_differentiable(out)
+        ctx.set_materialize_grads(False)  # (no zeros for `out`)
         return out[0], out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_loss, _):
+        if grad_loss is None:
+            return None, None, None, None, None, None
         log_prob, _, _, _, _, scratch = ctx.saved_tensors
         grad = torch.empty(log_prob.shape, device=log_prob.device, dtype=log_prob.dtype)
         if grad.numel() == 0:
@@ -182,8 +201,7 @@ def policy_loss(log_prob: torch.Tensor, advantage: torch.Tensor, old_log_prob: t
     packed, (x, adv, old, ref, mask) = _describe_policy(log_prob, advantage, old_log_prob, ref_log_prob, mask, clip_low, clip_high, dual_clip, kl_coef,
                                                         kl, reduction)
     if torch.is_grad_enabled() and log_prob.requires_grad:
-        const = [None if t is None else t.detach() for t in (adv, old, ref, mask)]
-        loss, out = _PolicyLoss.apply(x, *const, packed)
+        loss, out = _PolicyLoss.apply(x, _constant(adv), _constant(old), _constant(ref), mask, packed)
         return loss, _policy_info(out)
     out = torch.empty(5, device=x.device, dtype=torch.float32)
     scratch = _policy_scratch(x)
@@ -269,11 +287,14 @@ class _PreferenceLoss(torch.autograd.Function):
         ctx.save_for_backward(out, chosen_mask, rejected_mask)
         ctx.packed, ctx.shapes, ctx.dtype = packed, (chosen.shape, rejected.shape), chosen.dtype
         ctx.mark_non_differentiable(out)
+        ctx.set_materialize_grads(False)
         return out[0], out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_loss, _):
+        if grad_loss is None:
+            return None, None, None, None, None, None, None
         out = ctx.saved_tensors[0]
         gc, gr = (torch.empty(s, device=out.device, dtype=ctx.dtype) for s in ctx.shapes)
         scale = grad_loss.float()
@@ -298,8 +319,7 @@ def preference_loss(chosen: torch.Tensor, rejected: torch.Tensor, ref_chosen: to
     info                      accuracy (share of the pairs with h > 0), chosen_rewards and rejected_rewards (beta s, [pairs])"""
     packed, keep = _describe_preference(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, label_smoothing, kind, average)
     if torch.is_grad_enabled() and (chosen.requires_grad or rejected.requires_grad):
-        const = [None if t is None else t.detach() for t in (keep[1], keep[4], keep[2], keep[5])]
-        loss, out = _PreferenceLoss.apply(chosen, rejected, *const, packed)
+        loss, out = _PreferenceLoss.apply(chosen, rejected, _constant(keep[1]), _constant(keep[4]), keep[2], keep[5], packed)
     else:
         out, _, _ = _preference_forward(packed, chosen, rejected, False)
         loss = out[0]

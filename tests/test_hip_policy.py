@@ -561,3 +561,16 @@ def test_refusals():
     for args in ((u[0], None, u[0], dt), (u, u[:1], u, dt), (u, None, u.half(), dt), (u, None, u, dt[:1]), (u, None, u, dt.cpu()), (u[..., :0], None, u[..., :0], dt)):
         with pytest.raises(ValueError):
             P.step_log_ratio(*args)
+
+
+@gpu
+def test_gradients_are_differentiable_once():
+    x = torch.randn(3, 5, device="cuda", requires_grad=True)
+    u = torch.randn(3, 5, 2, device="cuda", requires_grad=True)
+    for f, t in ((lambda: P.policy_loss(x, torch.ones(3, device="cuda"))[0], x), (lambda: P.preference_loss(x, -x)[0], x),
+                 (lambda: P.step_log_ratio(u, None, u.detach(), torch.ones(3, device="cuda")).sum(), u)):
+        (first,) = torch.autograd.grad(f(), t)
+        (again,) = torch.autograd.grad(f(), t, create_graph=True)
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError):  # (a gradient of the gradient: there is none, and none is made up)
+            again.sum().backward()
