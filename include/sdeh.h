@@ -540,8 +540,8 @@ int32_t sdeh_importance_weights(const float* rnd, int64_t batch, const float* lo
  * ABI v8: losses over trajectories that were drawn before the update, and the update itself.
  *
  * Tensors of these entry points may be fp32, bf16 or fp16 (SdehDtype); sums, softmax-like statistics and optimizer moments are held in 32
- * or 64 bits whatever the inputs' type, every output is rounded once.  Nothing allocates or synchronises; scratch is the caller's and is
- * needed until the launches have run.  Captured into a graph, a replay reads the same pointers again.
+ * or 64 bits whatever the inputs' type, every output is rounded once.  Nothing allocates or synchronises; scratch is the caller's, aligned
+ * to 16 bytes, and needed until the launches have run.  Captured into a graph, a replay reads the same pointers again.
  */
 typedef enum { SDEH_F32 = 0, SDEH_BF16 = 1, SDEH_F16 = 2 } SdehDtype;
 
@@ -647,7 +647,7 @@ typedef struct {
   int32_t n_groups;
 } SdehAdamw;
 /* tensors: those of the first group, then those of the second, ..  They must not overlap, and no counter may serve two of them.
- * scratch: 16-byte aligned, sdeh_adamw_scratch_floats(all tensors). */
+ * scratch: sdeh_adamw_scratch_floats(all tensors). */
 int64_t sdeh_adamw_scratch_floats(int32_t n_tensors);
 int32_t sdeh_adamw_step(const SdehAdamw* p, const SdehAdamwGroup* groups, const SdehAdamwTensor* tensors, float* scratch, void* stream);
 /* The fp32 values that 8-bit moments stand for: `blocks` whole blocks of codes -> exp_avg, exp_avg_sq [blocks * SDEH_MOMENT_BLOCK] */

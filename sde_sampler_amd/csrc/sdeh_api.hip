@@ -2020,6 +2020,7 @@ int32_t sdeh_policy_loss(const SdehPolicyLoss* p, float* scratch, int32_t reuse_
     return fail(SDEH_ERR_INVALID, "policy_loss: unknown KL estimator or reduction");
   if (!(p->clip_low >= 0.0) || !(p->clip_high >= 0.0) || !(p->dual_clip == 0.0 || p->dual_clip > 1.0))
     return fail(SDEH_ERR_INVALID, "policy_loss: clip_low and clip_high are >= 0, dual_clip is 0 or > 1");
+  if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return fail(SDEH_ERR_INVALID, "policy_loss: scratch is not aligned to 16 bytes");
   const int rc = launch_policy_loss(*p, scratch, reuse_counts, grad_scale, grad_factor, out, grad, (hipStream_t)stream);
   return rc == SDEH_OK ? SDEH_OK : fail(rc, "policy_loss: launch failed");
 }
@@ -2045,6 +2046,7 @@ int32_t sdeh_preference_loss(const SdehPreferenceLoss* p, float* scratch, float 
   if (const int32_t bad = preference_ok(p); bad != SDEH_OK) return bad;
   if (scratch == nullptr || out == nullptr || (grad_chosen == nullptr) != (grad_rejected == nullptr))
     return fail(SDEH_ERR_INVALID, "preference_loss: null pointer");
+  if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return fail(SDEH_ERR_INVALID, "preference_loss: scratch is not aligned to 16 bytes");
   const int rc = launch_preference_loss(*p, scratch, grad_factor, out, grad_chosen, grad_rejected, (hipStream_t)stream);
   return rc == SDEH_OK ? SDEH_OK : fail(rc, "preference_loss: launch failed");
 }

@@ -81,7 +81,7 @@ class AdamW(torch.optim.Optimizer):
 
     `lr` may be a one-element fp32 tensor on the parameters' device (a schedule under a captured graph).  A step never synchronises and may be
     captured (utils/graphs.py: GraphedTrainStep).  Parameters are contiguous fp32, bf16 or fp16 tensors on one HIP device; those without a gradient
-    are left alone."""
+    are left alone.  Parameters must not share memory.  A parameter group added later moves the moments: capture again."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, *, state_bits: int = 32,
                  max_grad_norm: float | None = None, seed: int = 0):
@@ -124,7 +124,7 @@ class AdamW(torch.optim.Optimizer):
         """[(group, its buckets)]; flat state buffers are made here and take over what `self.state` holds."""
         if self._buckets is not None:
             return self._buckets
-        plan, first, device = [], 0, None
+        plan, first, device, seen = [], 0, None, set()
         for group in self.param_groups:
             by_type: dict = {}
             for p in group["params"]:
@@ -135,6 +135,9 @@ class AdamW(torch.optim.Optimizer):
                 if device is not None and p.device != device:
                     raise L.SdehUnsupported(-2, f"AdamW: parameters on {device} and {p.device} (one optimizer, one device)")
                 device = p.device
+                if id(p) in seen:
+                    raise ValueError("AdamW: a parameter is there twice")
+                seen.add(id(p))
                 by_type.setdefault(p.dtype, []).append(p)
             buckets = []
             for params in by_type.values():
@@ -207,7 +210,7 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, closure=None, *, ok: torch.Tensor | None = None):
         """One step.  ok: an optional one-element bool tensor on the device; where it is False, parameters, moments and step counters stay as they are
-        (the decision of `if loss_ok and grad_ok`, solver/base.py:409-421, without a host round trip)."""
+        (the decision of `if loss_ok and grad_ok`, solver/base.py:409-421, without a host round trip), and `grad_norm` too."""
         loss = None
         if closure is not None:
             with torch.enable_grad():

@@ -527,6 +527,10 @@ def test_c_entry_refuses_bad_arguments():
 
 @gpu
 def test_step_refuses():
+    q = torch.nn.Parameter(torch.zeros(5, device="cuda"))
+    q.grad = torch.ones_like(q)
+    with pytest.warns(UserWarning, match="duplicate"), pytest.raises(ValueError, match="twice"):
+        AdamW([q, q]).step()
     p = torch.nn.Parameter(torch.zeros(4, 6, device="cuda"))
     opt = AdamW([p])
     p.grad = torch.ones_like(p)

@@ -255,6 +255,18 @@ def test_policy_loss_layouts(R, T, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("R,T", [(5, 64), (41, 1003)])
+def test_masks_of_any_nonzero_byte(R, T):
+    lp, old, ref, adv, m = (t.cuda() for t in _policy_case(R, T, torch.float32, "random", "rows"))
+    bytes_ = m.to(torch.uint8) * torch.randint(1, 256, m.shape, device="cuda", dtype=torch.uint8)
+    for reduction in ("steps", "rows"):
+        a, b = (P.policy_loss_and_grad(lp, adv, old, ref, k, reduction=reduction, kl_coef=0.1) for k in (m, bytes_))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2])
+    a, b = (P.preference_loss_and_grad(lp, old, None, None, k, k) for k in (m, bytes_))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2]) and torch.equal(a[3], b[3])
+
+
+@gpu
 def test_policy_loss_borders_and_extremes():
     """Either side of the clipping borders by one step of fp32, no clipping at all, ratios that overflow, empty tensors."""
     hi, lo = math.log1p(0.28), math.log1p(-0.2)
@@ -509,7 +521,7 @@ def test_c_entries_refuse_bad_arguments():
     ok = lambda **k: L.POLICY_LOSS.pack(*(64, 4, 1) * 5, k.get("rows", 2), k.get("steps", 4), k.get("dtype", 0), 0, k.get("kl", 3), k.get("red", 0),  # noqa: E731
                                         k.get("lo", 0.2), k.get("hi", 0.2), k.get("dual", 0.0), 0.0)
     call = lambda p, s=64, o=64, g=None: lib.sdeh_policy_loss(p, s, 0, None, 1.0, o, g, None)  # noqa: E731
-    assert call(None) == call(ok(), s=None) == call(ok(), o=None) == -1
+    assert call(None) == call(ok(), s=None) == call(ok(), s=72) == call(ok(), o=None) == -1
     for bad in (dict(rows=-1), dict(steps=-1), dict(steps=1 << 31), dict(rows=1 << 40, steps=1 << 30), dict(dtype=3), dict(kl=0), dict(red=3),
                 dict(lo=-0.1), dict(hi=math.nan), dict(dual=0.5)):
         assert call(ok(**bad)) == -1, bad
@@ -521,6 +533,7 @@ def test_c_entries_refuse_bad_arguments():
     for bad in (dict(pairs=0), dict(dtype=-1), dict(kind=3), dict(beta=0.0), dict(beta=math.nan), dict(eps=0.5), dict(c=(0,) * 9 + (4,)),
                 dict(c=(64, 4, 1) + (0,) * 6 + (-1,))):
         assert lib.sdeh_preference_loss(pref(**bad), 64, 1.0, 64, None, None, None) == -1, bad
+    assert lib.sdeh_preference_loss(pref(), 72, 1.0, 64, None, None, None) == -1
     assert lib.sdeh_preference_loss(pref(), None, 1.0, 64, None, None, None) == lib.sdeh_preference_loss(pref(), 64, 1.0, 64, 64, None, None) == -1
     assert lib.sdeh_preference_grad(pref(), 64, None, 1.0, None, 64, None) == -1
     assert lib.sdeh_step_log_ratio(64, None, 64, 64, 2, 2, 0, 0, 64, None) == lib.sdeh_step_log_ratio(64, None, None, 64, 2, 2, 2, 0, 64, None) == -1

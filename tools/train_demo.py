@@ -26,6 +26,7 @@ def main():
     ap.add_argument("--no-guard", action="store_true", help="with --graph: no device-side skip of non-finite updates")
     ap.add_argument("--em-steps", type=int, default=None, help="Euler-Maruyama steps of the grid (default: the specification's)")
     ap.add_argument("--channels", type=int, default=None, help="network width (default: the specification's)")
+    ap.add_argument("--state-bits", type=int, choices=(8, 32), default=None, help="train with utils.optim.AdamW, moments in this many bits")
     ap.add_argument("--print-every", type=int, default=100)
     args = ap.parse_args()
     if args.name == "bridge_dw":  # a Bridge (conf/solver/bridge.yaml style) on the shifted double well
@@ -54,7 +55,16 @@ def main():
         inf_params = list(prob.loss.inference_ctrl.parameters())
         groups.append(dict(params=inf_params, lr=0.02 * args.lr))
         train_params = train_params + inf_params
-    opt = torch.optim.Adam(groups, capturable=args.graph, fused=args.graph)  # (fused: one launch; the capturable foreach form runs ~90 per-tensor kernels)
+    if args.state_bits:  # this package's optimizer: clipping, the update and -- under the graph's guard -- skipping it in two launches
+        from sde_sampler_amd.utils.optim import AdamW
+
+        opt = AdamW(groups, weight_decay=0.0, state_bits=args.state_bits, max_grad_norm=1.0)
+    else:
+        opt = torch.optim.Adam(groups, capturable=args.graph, fused=args.graph)  # (fused: one launch; the capturable foreach form runs ~90 per-tensor kernels)
+
+    def clip():
+        if not args.state_bits:
+            torch.nn.utils.clip_grad_norm_(train_params, 1.0)
 
     def evaluate(tag):
         x = prob.prior.sample((args.eval_batch,))
@@ -75,8 +85,7 @@ def main():
             x = prob.prior.sample((args.batch,))
             return prob.loss(prob.ts, x, prob.target.unnorm_log_prob, prob.second_log_prob)[0]
 
-        graphed = GraphedTrainStep(loss_fn, [prob.loss], opt, warmup=3, guard=not args.no_guard,
-                                   after_backward=lambda: torch.nn.utils.clip_grad_norm_(train_params, 1.0))
+        graphed = GraphedTrainStep(loss_fn, [prob.loss], opt, warmup=3, guard=not args.no_guard, after_backward=clip)
     t0 = t_last = time.perf_counter()
     for step in range(args.steps):
         if graphed is not None:
@@ -86,7 +95,7 @@ def main():
             loss, _ = prob.loss(prob.ts, x, prob.target.unnorm_log_prob, prob.second_log_prob)
             opt.zero_grad(set_to_none=True)
             loss.backward()
-            torch.nn.utils.clip_grad_norm_(train_params, 1.0)
+            clip()
             opt.step()
         if (step + 1) % args.print_every == 0:
             torch.cuda.synchronize()
