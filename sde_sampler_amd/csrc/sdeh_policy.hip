@@ -27,6 +27,7 @@ __device__ __forceinline__ void split_index(long long i, long long steps, long l
 // A row is one trajectory at one step, dim coordinates: 1 .. a few hundred, seldom a multiple of what a lane loads at once.  A workgroup
 // therefore takes `rows` whole rows -- one contiguous stretch, loaded 16 bytes a lane whatever dim is --, puts the elements' terms into LDS and
 // sums the rows from there with G lanes a row.  dt differs from row to row only where a stretch passes the end of a step; it is staged per row.
+// Bounded by memory: 200 x 4096 x 196 bf16 forward 0.18 ms (0.96 GB, 5.4 TB/s), backward 0.22 ms (1.28 GB, 5.9 TB/s); 200 x 2048 x 50 fp32 54 + 52 us.
 // -------------------------------------------------------------------------------------------------------------------------------------------
 constexpr int kStretch = 4096;      // elements of a stretch, at most (16 KB of terms)
 constexpr int kStretchRows = 1024;  // rows of a stretch, at most
@@ -280,6 +281,8 @@ namespace {
 // entry, i.e. how many entries are valid -- a pass over the mask's bytes alone (1 of 14 to 21 bytes an entry), which leaves partial counts that
 // every workgroup of the main pass adds up again.  No atomics, no last-workgroup ticket: results do not depend on the order of workgroups and
 // nothing has to be cleared between calls.
+// 8192 x 8191 bf16 entries with a KL term and an advantage each, 62 % valid: 17 us for the mask, 131 us for the pass -- 0.6 GB, 100 us at the rate of a
+// large copy; 60 vector instructions an entry take 76 us of it --, 5 us for the result.
 // -------------------------------------------------------------------------------------------------------------------------------------------
 constexpr int kCountBlocks = 1024, kPolicyBlocks = 2048, kSmallThreads = 1024;
 
@@ -736,7 +739,8 @@ __global__ __launch_bounds__(kSmallThreads) void policy_small_kernel(PolicyArgs 
   if (threadIdx.x == 0) policy_result(a, policy, kl, (double)clipped, (double)valid);
 }
 
-constexpr long long kPolicySmall = 8192;  // entries that one workgroup takes
+// Entries that one workgroup takes, in one launch: 1600 of them 7 us; three launches of 2.5 to 5 us otherwise, and twice the time on the host.
+constexpr long long kPolicySmall = 8192;
 
 bool dense(const SdehPlane& q, long long steps, size_t bytes) {
   return q.data == nullptr || (q.step_stride == 1 && q.row_stride == steps && aligned_to(q.data, bytes));
@@ -821,7 +825,8 @@ namespace {
 // preference loss: sums of the rows (split over their length where rows are few and long), the pairs, the gradients
 //
 // A pair's slope is known only when both its rows are summed, so the gradient -- the slope again and again, 0 in the padding -- is a second
-// pass; it reads nothing but the mask.
+// pass; it reads nothing but the mask.  24 pairs of 2.6e5 and 2.0e5 fp16 entries: sums 15 us, pairs 5, gradients 9 (77 MB, 12 us at the rate of a large
+// copy); below 8192 entries everything in one launch, 8 us.
 // -------------------------------------------------------------------------------------------------------------------------------------------
 constexpr int kPairBlocks = 256;
 
