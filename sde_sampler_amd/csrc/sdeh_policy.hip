@@ -739,8 +739,9 @@ __global__ __launch_bounds__(kSmallThreads) void policy_small_kernel(PolicyArgs 
   if (threadIdx.x == 0) policy_result(a, policy, kl, (double)clipped, (double)valid);
 }
 
-// Entries that one workgroup takes, in one launch: 1600 of them 7 us; three launches of 2.5 to 5 us otherwise, and twice the time on the host.
-constexpr long long kPolicySmall = 8192;
+// Entries that one workgroup takes, in one launch.  Replayed from a graph, fp32 with a mask and row weights: 1024 entries 10.7 us, 4096 13.1, 8192 17.3;
+// in three launches 12.0 us from 16384 on (without a mask 7.1, 7.9, 9.6; in two launches 7.6).  On the host each launch less saves 3 us.
+constexpr long long kPolicySmall = 4096;
 
 bool dense(const SdehPlane& q, long long steps, size_t bytes) {
   return q.data == nullptr || (q.step_stride == 1 && q.row_stride == steps && aligned_to(q.data, bytes));
@@ -826,7 +827,7 @@ namespace {
 //
 // A pair's slope is known only when both its rows are summed, so the gradient -- the slope again and again, 0 in the padding -- is a second
 // pass; it reads nothing but the mask.  24 pairs of 2.6e5 and 2.0e5 fp16 entries: sums 15 us, pairs 5, gradients 9 (77 MB, 12 us at the rate of a large
-// copy); below 8192 entries everything in one launch, 8 us.
+// copy); up to 4096 entries everything in one launch, 6 to 9 us.
 // -------------------------------------------------------------------------------------------------------------------------------------------
 constexpr int kPairBlocks = 256;
 
@@ -1130,7 +1131,8 @@ __global__ __launch_bounds__(kSmallThreads) void preference_small_kernel(Prefere
   }
 }
 
-constexpr long long kPreferenceSmall = 8192;  // entries of both sides that one workgroup takes
+// Entries of both sides that one workgroup takes, in one launch: 1024 entries 6.4 us, 4096 8.5, 8192 11.6; in three launches 7.6 us from 16384 on.
+constexpr long long kPreferenceSmall = 4096;
 constexpr long long kShortRow = 1024;         // rows that a wave sums
 constexpr int kMaxSplits = 64;
 
