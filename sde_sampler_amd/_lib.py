@@ -230,6 +230,7 @@ PROTOTYPES = {
 }
 
 _LIB = None
+_TORCH = None
 
 
 def library_path() -> Path:
@@ -239,11 +240,12 @@ def library_path() -> Path:
 
 def load():
     """Loads libsdeh.so once (after torch, so that it binds to the HIP runtime torch already loaded)."""
-    global _LIB
+    global _LIB, _TORCH
     if _LIB is not None:
         return _LIB
-    import torch  # noqa: F401  (must come first: one HIP runtime per process)
+    import torch  # (must come first: one HIP runtime per process)
 
+    _TORCH = torch
     path = library_path()
     if not path.exists():
         raise SdehLibraryError(
@@ -284,14 +286,12 @@ def call(name: str, device, *args):
     fn = _FUNCTIONS.get(name)
     if fn is None:
         fn = _FUNCTIONS[name] = getattr(load(), name)
-    from torch import _C, cuda
-
     index = device.index
-    if _C._cuda_getDevice() == index:
-        status = fn(*args, _C._cuda_getCurrentRawStream(index))
+    if _TORCH._C._cuda_getDevice() == index:
+        status = fn(*args, _TORCH._C._cuda_getCurrentRawStream(index))
     else:
-        with cuda.device(index):
-            status = fn(*args, _C._cuda_getCurrentRawStream(index))
+        with _TORCH.cuda.device(index):
+            status = fn(*args, _TORCH._C._cuda_getCurrentRawStream(index))
     if status != 0:
         check(status)
 

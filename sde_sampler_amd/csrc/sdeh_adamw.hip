@@ -410,7 +410,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(Batch b, Common a) {
   }
 }
 
-// 10 bytes an entry, 8 of them written: 100 M entries in 0.18 ms, 5.5 TB/s
+// 10 bytes an entry, 8 of them written: 100 M entries in 0.2 ms, 5 TB/s
+template <bool STREAM>
 __global__ __launch_bounds__(kThreads) void adamw_moments_kernel(const uint8_t* __restrict__ m, const uint8_t* __restrict__ m_top,
                                                                  const uint8_t* __restrict__ v, const uint8_t* __restrict__ v_top, long long n,
                                                                  float* __restrict__ om, float* __restrict__ ov) {
@@ -424,8 +425,8 @@ __global__ __launch_bounds__(kThreads) void adamw_moments_kernel(const uint8_t* 
       xm[e] = from_code<true>(km >> (8 * e) & 255u, bm);
       xv[e] = from_code<false>(kv >> (8 * e) & 255u, bv);
     }
-    store_pack<float, 4>(om + i, xm);
-    store_pack<float, 4>(ov + i, xv);
+    put<float, STREAM>(om + i, xm);
+    put<float, STREAM>(ov + i, xv);
   }
 }
 
@@ -535,7 +536,11 @@ int launch_adamw_step(const SdehAdamw& p, const SdehAdamwGroup* groups, const Sd
 int launch_adamw_moments(const uint8_t* m, const uint8_t* m_top, const uint8_t* v, const uint8_t* v_top, long long blocks, float* om, float* ov,
                          hipStream_t stream) {
   const long long n = blocks * kBlock, wanted = (n / 4 + kThreads - 1) / kThreads;
-  hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)(wanted < 4096 ? wanted : 4096)), dim3(kThreads), 0, stream, m, m_top, v, v_top, n, om, ov);
+  const dim3 grid((unsigned)(wanted < 4096 ? wanted : 4096));
+  if (n * 8 > kCacheBytes)  // (100 M entries, step and values together: 460 us through the caches, 439 past them)
+    hipLaunchKernelGGL(adamw_moments_kernel<true>, grid, dim3(kThreads), 0, stream, m, m_top, v, v_top, n, om, ov);
+  else
+    hipLaunchKernelGGL(adamw_moments_kernel<false>, grid, dim3(kThreads), 0, stream, m, m_top, v, v_top, n, om, ov);
   return hipGetLastError() == hipSuccess ? SDEH_OK : SDEH_ERR_HIP;
 }
 
