@@ -1,8 +1,8 @@
 // One AdamW step over many tensors, moments in 32 or in 8 bits, gradients clipped by their global norm (include/sdeh.h, ABI v8).
 //
 // With 32-bit moments bounded by memory: fp32 reads and writes 28 bytes an entry (and the gradient's 4 once more for the norm); 150 M entries take
-// 0.80 ms (5.3 TB/s; a large elementwise kernel reaches 6.2) after 0.12 ms for the norm.  With 8-bit moments it is 10 bytes of bf16 (and 2) but 68
-// vector instructions an entry -- codes, two hashed roundings, the update --: 100 M entries take 0.22 ms, of which the instructions alone 0.19, and the
+// 0.78 ms (5.4 TB/s; a large elementwise kernel reaches 6.2) after 0.12 ms for the norm.  With 8-bit moments it is 10 bytes of bf16 (and 2) but some 65
+// vector instructions an entry -- codes, two hashed roundings, the update --: 100 M entries take 0.21 ms, of which the instructions alone 0.17, and the
 // norm 0.04.  Small models are bounded by two launches, 9 us.  Two launches for each 48 tensors: the first forms partial sums of the gradients' squares and the tensors' coefficients
 // (step counters, bias corrections), the second adds the partial sums up again in every workgroup -- 2048 doubles from L2 -- and updates.  The
 // tensors' pointers travel as kernel arguments: no table on the device, nothing to keep or to invalidate.
@@ -153,12 +153,24 @@ __device__ __forceinline__ float product(float x, float y) {
   return x * y;
 }
 
-// The hardware's square root and reciprocal (one unit in the last place each) are enough for an update that is lr times smaller than what it is added to;
-// its square root takes no subnormal numbers: those are scaled.
-__device__ __forceinline__ float new_param(float p, float m, float v, const Coef& c, float eps) {
-  const bool low = v < 0x1p-96f;
-  const float root = __builtin_amdgcn_sqrtf(low ? v * 0x1p64f : v) * (low ? 0x1p-32f : 1.0f);
-  return fmaf(p, c.decay, -c.step_size * (m * __builtin_amdgcn_rcpf(fmaf(root, c.inv_root, eps))));
+// The hardware's square root and reciprocal (one unit in the last place each) are enough for an update that is lr times smaller than what it is added to.
+// Its square root may take a subnormal number for 0, i.e. be off by 2^-63: beside an eps of kPlainRoots or more that is nothing; below, small numbers are
+// scaled first.
+constexpr float kPlainRoots = 1e-11f;
+__device__ __forceinline__ void new_params(float (&p)[4], const float (&m)[4], const float (&v)[4], const Coef& c, float eps) {
+  float root[4];
+  if (eps >= kPlainRoots) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) root[e] = __builtin_amdgcn_sqrtf(v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool low = v[e] < 0x1p-96f;
+      root[e] = __builtin_amdgcn_sqrtf(low ? v[e] * 0x1p64f : v[e]) * (low ? 0x1p-32f : 1.0f);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) p[e] = fmaf(p[e], c.decay, -c.step_size * (m[e] * __builtin_amdgcn_rcpf(fmaf(root[e], c.inv_root, eps))));
 }
 
 // the largest value of a wave, in a scalar register (shifts within rows of 16 lanes, then rows to rows; 0 comes in from outside)
@@ -190,10 +202,15 @@ __device__ __forceinline__ unsigned to_codes(const unsigned (&q)[4], const float
     const unsigned bits = __float_as_uint(x[e]);
     unsigned c;
     if (SIGNED)
-      c = (unsigned)clamp_int((int)q[e] - base, 0, 127) | (bits >> 24 & 128u);  // (127 cuts a NaN whose payload is all ones)
+      c = (unsigned)clamp_int((int)q[e] - base, 0, 127);  // (127 cuts a NaN whose payload is all ones)
     else
       c = (bits & 0x7FFFFFFFu) == 0u ? 0u : (unsigned)clamp_int((int)q[e] - base, 1, 255);  // (a second moment above 0 stays above 0: it divides)
     out |= c << (8 * e);
+  }
+  if (SIGNED) {  // the four top bytes side by side; of each its sign
+    const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x0C0C0703u);
+    const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x07030C0Cu);
+    out |= (lo | hi) & 0x80808080u;
   }
   return out;
 }
@@ -238,7 +255,7 @@ struct Four {
     const P* tg = static_cast<const P*>(t.g) + i;
     if (FAST) {
       get<P, STREAM>(tp, p);
-      load_pack<P, 4>(tg, g);
+      get<P, STREAM>(tg, g);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -295,8 +312,8 @@ struct Four {
       const float y = product(g[e], scale);  // (scale is 1 without clipping: exact)
       m[e] = blend(a.beta1, m[e], a.rest1, y);
       v[e] = blend(a.beta2, v[e], a.rest2, product(y, y));
-      p[e] = new_param(p[e], m[e], v[e], c, a.eps);
     }
+    new_params(p, m, v, c, a.eps);
     P* tp = static_cast<P*>(t.p) + i;
     if (FAST) {
       put<P, STREAM>(tp, p);
@@ -385,14 +402,16 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(Batch b, Common a) {
                       ((reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) & (BITS == 8 ? 3 : 15)) == 0;
     long long j = at + kBlock * wave;
     if (wide) {
-      // two blocks at a time: both blocks' loads are on their way before the first is computed
-      for (; j + kThreads * 4 + kBlock <= end; j += 2 * kThreads * 4) {
-        Four<P, BITS, STREAM> x, y;
+      // four blocks at a time: all their loads are on their way before the first is computed (two at a time: 0.80 ms instead of 0.78 for 150 M fp32 entries
+      // with 32-bit moments, 0.23 instead of 0.21 for 100 M of bf16 with 8-bit ones)
+      constexpr int U = 4, kStep = kThreads * 4;
+      for (; j + (U - 1) * kStep + kBlock <= end; j += U * kStep) {
+        Four<P, BITS, STREAM> x[U];
         const long long i = j + 4 * lane;
-        x.template load<true>(t, i, 4);
-        y.template load<true>(t, i + kThreads * 4, 4);
-        x.template update<true>(t, a, coef, scale, i, 4);
-        y.template update<true>(t, a, coef, scale, i + kThreads * 4, 4);
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u].template load<true>(t, i + u * kStep, 4);
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u].template update<true>(t, a, coef, scale, i + u * kStep, 4);
       }
     }
     for (; j < end; j += kThreads * 4) {
@@ -468,7 +487,7 @@ int launch_adamw_step(const SdehAdamw& p, const SdehAdamwGroup* groups, const Sd
   // small units while there are not enough of them to go round (13 tensors of a 64-channel network: 5.3 us in units of 1024, 7.4 in units of 4096;
   // above 2 M entries a unit's start costs more than the balance gives)
   const int chunk = entries <= 2048ll * 1024 ? 1024 : 8192;
-  // what does not fit the 256 MB cache anyway goes past it and leaves it to the gradients, which are read twice (150 M fp32 entries: update 826 -> 800 us,
+  // what does not fit the 256 MB cache anyway goes past it and leaves it to the gradients, which are read twice (150 M fp32 entries: update 826 -> 790 us,
   // norm 158 -> 118); smaller states stay in it from step to step
   const bool past_caches = bytes > kCacheBytes;
   // pass 0: refuse what does not fit, before anything runs; pass 1: coefficients and norm; pass 2: update

@@ -184,6 +184,26 @@ def test_step(dtype, clip, unaligned, bits):
 
 
 @gpu
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-12, 1e-8])
+def test_tiny_gradients(eps):
+    """Second moments down to the subnormal numbers: sqrt(v) counts beside whatever eps there is."""
+    p = torch.nn.Parameter(torch.ones(4096, device="cuda"))
+    g = torch.full((4096,), 10.0).pow(torch.linspace(-24, -3, 4096))
+    opt = AdamW([p], lr=0.5, eps=eps, weight_decay=0.0)
+    p.grad = g.cuda()
+    opt.step()
+    s = {k: t.cpu() for k, t in opt.state[p].items()}
+    # from the moments as they are held (g^2 below 1e-38 has few digits left, below 1e-45 none)
+    denom = s["exp_avg_sq"].double().sqrt() / math.sqrt(1 - 0.999) + eps
+    want = 1.0 - 0.5 / (1 - 0.9) * s["exp_avg"].double() / denom
+    some = denom > 0
+    assert some.sum() > 3000
+    # sqrt, reciprocal, three products, two coefficients and two sums: below 20 roundings; a root taken for 0 is below 2^-63, 2^-58 with its bias correction
+    tol = 20 * H * (1.0 + (want - 1.0).abs()) + ((want - 1.0).abs() * 2.0 ** -58 / eps if eps >= 1e-11 else 0.0)
+    assert ((p.detach().cpu().double() - want).abs() <= tol)[some].all()
+
+
+@gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_moments_are_the_states_values(bits):
     params = _params(SIZES, torch.float32)
