@@ -60,7 +60,7 @@ class _Bucket:
             if g.is_sparse or g.get_device() != index or g.dtype != dtype or g.numel() != n:
                 raise RuntimeError("AdamW: gradients must be dense and of their parameter's type, size and device")
             if not g.is_contiguous():
-                g = g.contiguous()
+                g = g.detach().contiguous()
                 keep.append(g)
             param.append(p.data_ptr())
             grad.append(g.data_ptr())
@@ -207,7 +207,6 @@ class AdamW(torch.optim.Optimizer):
         return tuple(torch.cat([f[k] for f in flats]) for k in (0, 1))
 
     # -- step ----------------------------------------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, closure=None, *, ok: torch.Tensor | None = None):
         """One step.  ok: an optional one-element bool tensor on the device; where it is False, parameters, moments and step counters stay as they are
         (the decision of `if loss_ok and grad_ok`, solver/base.py:409-421, without a host round trip), and `grad_norm` too."""
