@@ -110,7 +110,7 @@ def _plane(t: torch.Tensor | None):
 
 
 def _describe_policy(log_prob, advantage, old, ref, mask, clip_low, clip_high, dual_clip, kl_coef, kl, reduction):
-    """(packed SdehPolicyLoss, the tensors it points at)"""
+    """(the tensors as the kernel takes them, the rest of SdehPolicyLoss)"""
     if log_prob.ndim != 2:
         raise ValueError(f"policy_loss: log_prob must be [rows, steps], got {tuple(log_prob.shape)}")
     dev, shape = log_prob.device, log_prob.shape
@@ -120,13 +120,10 @@ def _describe_policy(log_prob, advantage, old, ref, mask, clip_low, clip_high, d
             raise ValueError(f"policy_loss: {name} is {tuple(t.shape)} {t.dtype} on {t.device}, log_prob {tuple(shape)} {log_prob.dtype} on {dev}")
     adv_code = _code("policy_loss", advantage, dev)
     try:
-        if advantage.ndim == 1 and advantage.shape[0] == shape[0]:
-            adv_plane = (advantage.data_ptr(), advantage.stride(0), 0)
-        elif advantage.ndim == 2:
+        if advantage.ndim == 2:
             if advantage.shape != shape:
                 advantage = advantage.expand(shape)
-            adv_plane = _plane(advantage)
-        else:
+        elif advantage.ndim != 1 or advantage.shape[0] != shape[0]:
             raise ValueError(f"policy_loss: advantage must be [rows] or [rows, steps], got {tuple(advantage.shape)} for log_prob {tuple(shape)}")
         if mask is not None and mask.shape != shape:
             mask = mask.expand(shape)
@@ -138,9 +135,14 @@ def _describe_policy(log_prob, advantage, old, ref, mask, clip_low, clip_high, d
         raise ValueError(f"policy_loss: kl is one of {list(L.KL_ESTIMATORS)} and reduction one of {list(L.REDUCTIONS)}, got {kl!r} and {reduction!r}")
     if not (clip_low >= 0.0 and clip_high >= 0.0 and (dual_clip is None or dual_clip > 1.0)):
         raise ValueError(f"policy_loss: clip_low, clip_high >= 0 and dual_clip > 1, got {clip_low}, {clip_high}, {dual_clip}")
-    p = L.POLICY_LOSS.pack(*_plane(log_prob), *_plane(old), *_plane(ref), *adv_plane, *_plane(mask), *shape, code, adv_code,
-                           L.KL_ESTIMATORS[kl], L.REDUCTIONS[reduction], clip_low, clip_high, dual_clip or 0.0, kl_coef)
-    return p, (log_prob, advantage, old, ref, mask)
+    rest = (*shape, code, adv_code, L.KL_ESTIMATORS[kl], L.REDUCTIONS[reduction], clip_low, clip_high, dual_clip or 0.0, kl_coef)
+    return (log_prob, advantage, old, ref, mask), rest
+
+
+def _pack_policy(tensors, rest) -> bytes:
+    log_prob, advantage, old, ref, mask = tensors
+    adv = (advantage.data_ptr(), advantage.stride(0), 0) if advantage.ndim == 1 else _plane(advantage)
+    return L.POLICY_LOSS.pack(*_plane(log_prob), *_plane(old), *_plane(ref), *adv, *_plane(mask), *rest)
 
 
 def _policy_scratch(log_prob):
@@ -157,12 +159,13 @@ class _PolicyLoss(torch.autograd.Function):
     scaled loss (gradient accumulation, half-precision loss scaling) loses nothing."""
 
     @staticmethod
-    def forward(ctx, log_prob, advantage, old, ref, mask, packed):
+    def forward(ctx, log_prob, advantage, old, ref, mask, rest):
         scratch = _policy_scratch(log_prob)
         out = torch.empty(5, device=log_prob.device, dtype=torch.float32)
+        packed = _pack_policy((log_prob, advantage, old, ref, mask), rest)
         L.call("sdeh_policy_loss", log_prob.device, packed, scratch.data_ptr(), 0, None, 1.0, out.data_ptr(), None)
         ctx.save_for_backward(log_prob, advantage, old, ref, mask, scratch)
-        ctx.packed = packed
+        ctx.rest, ctx.mask_stride = rest, None if mask is None else mask.stride()
         ctx.mark_non_differentiable(out)
         ctx.set_materialize_grads(False)  # (no zeros for `out`)
         return out[0], out
@@ -172,12 +175,14 @@ class _PolicyLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, _):
         if grad_loss is None:
             return None, None, None, None, None, None
-        log_prob, _, _, _, _, scratch = ctx.saved_tensors
+        *tensors, scratch = ctx.saved_tensors  # (they may have been away: their addresses are taken anew)
+        log_prob, mask = tensors[0], tensors[4]
+        counted = mask is None or mask.stride() == ctx.mask_stride  # (the counts in `scratch` are those of the mask's layout)
         grad = torch.empty(log_prob.shape, device=log_prob.device, dtype=log_prob.dtype)
         if grad.numel() == 0:
             return grad, None, None, None, None, None
         scale = grad_loss.float()
-        L.call("sdeh_policy_loss", log_prob.device, ctx.packed, scratch.data_ptr(), 1, scale.data_ptr(), 1.0, None, grad.data_ptr())
+        L.call("sdeh_policy_loss", log_prob.device, _pack_policy(tensors, ctx.rest), scratch.data_ptr(), int(counted), scale.data_ptr(), 1.0, None, grad.data_ptr())
         return grad, None, None, None, None, None
 
 
@@ -198,11 +203,12 @@ def policy_loss(log_prob: torch.Tensor, advantage: torch.Tensor, old_log_prob: t
     reduction     "steps": mean over the valid entries; "rows": mean over the rows that have any, of their means; "sum"
     info          0-d fp32 tensors: policy and kl (the two terms, reduced like the loss), clip_fraction, n_valid
     Without a valid entry the loss and its gradient are 0.  A log-probability of -inf in a valid entry gives what the formula gives."""
-    packed, (x, adv, old, ref, mask) = _describe_policy(log_prob, advantage, old_log_prob, ref_log_prob, mask, clip_low, clip_high, dual_clip, kl_coef,
-                                                        kl, reduction)
+    tensors, rest = _describe_policy(log_prob, advantage, old_log_prob, ref_log_prob, mask, clip_low, clip_high, dual_clip, kl_coef, kl, reduction)
+    x, adv, old, ref, mask = tensors
     if torch.is_grad_enabled() and log_prob.requires_grad:
-        loss, out = _PolicyLoss.apply(x, _constant(adv), _constant(old), _constant(ref), mask, packed)
+        loss, out = _PolicyLoss.apply(x, _constant(adv), _constant(old), _constant(ref), mask, rest)
         return loss, _policy_info(out)
+    packed = _pack_policy(tensors, rest)
     out = torch.empty(5, device=x.device, dtype=torch.float32)
     scratch = _policy_scratch(x)
     L.call("sdeh_policy_loss", x.device, packed, scratch.data_ptr(), 0, None, 1.0, out.data_ptr(), None)
@@ -215,8 +221,9 @@ def policy_loss_and_grad(log_prob: torch.Tensor, advantage: torch.Tensor, old_lo
                          grad_scale: float = 1.0) -> tuple[torch.Tensor, dict, torch.Tensor]:
     """`policy_loss` and grad_scale * d loss / d log_prob from one pass over the inputs, without an autograd graph: (loss, info, gradient).
     `log_prob.backward(gradient)` hands it to whatever computed log_prob."""
-    packed, (x, *keep) = _describe_policy(log_prob.detach(), advantage, old_log_prob, ref_log_prob, mask, clip_low, clip_high, dual_clip, kl_coef, kl,
-                                          reduction)
+    tensors, rest = _describe_policy(log_prob.detach(), advantage, old_log_prob, ref_log_prob, mask, clip_low, clip_high, dual_clip, kl_coef, kl,
+                                     reduction)
+    x, packed = tensors[0], _pack_policy(tensors, rest)
     out = torch.empty(5, device=x.device, dtype=torch.float32)
     grad = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     scratch = _policy_scratch(x)
@@ -230,7 +237,7 @@ def _describe_preference(chosen, rejected, ref_chosen, ref_rejected, chosen_mask
         raise ValueError(f"preference_loss: chosen and rejected must be [pairs, steps] with as many (and at least one) pairs, got {tuple(chosen.shape)} "
                          f"and {tuple(rejected.shape)}")
     code = _code("preference_loss", chosen)
-    sides, tensors = [], []
+    tensors = []
     for name, x, ref, mask in (("chosen", chosen, ref_chosen, chosen_mask), ("rejected", rejected, ref_rejected, rejected_mask)):
         if x.dtype != chosen.dtype or x.device != chosen.device:
             raise ValueError(f"preference_loss: chosen is {chosen.dtype} on {chosen.device}, rejected {x.dtype} on {x.device}")
@@ -245,7 +252,6 @@ def _describe_preference(chosen, rejected, ref_chosen, ref_rejected, chosen_mask
                     mask = mask.expand(x.shape)
                 except RuntimeError as exc:
                     raise ValueError(f"preference_loss: {name}_mask must broadcast to {tuple(x.shape)}: {exc}") from None
-        sides += [*_plane(x), *_plane(ref), *_plane(mask), x.shape[1]]
         tensors += [x, ref, mask]
     if kind not in L.PREFERENCE_KINDS:
         raise ValueError(f"preference_loss: kind is one of {list(L.PREFERENCE_KINDS)}, got {kind!r}")
@@ -253,8 +259,12 @@ def _describe_preference(chosen, rejected, ref_chosen, ref_rejected, chosen_mask
         raise ValueError(f"preference_loss: beta > 0 and 0 <= label_smoothing < 0.5, got {beta} and {label_smoothing}")
     if label_smoothing and kind != "logistic":
         raise ValueError(f"preference_loss: label_smoothing belongs to the logistic kind, got {kind!r}")
-    p = L.PREFERENCE_LOSS.pack(*sides, chosen.shape[0], code, L.PREFERENCE_KINDS[kind], bool(average), beta, label_smoothing)
-    return p, tensors
+    return tensors, (chosen.shape[0], code, L.PREFERENCE_KINDS[kind], bool(average), beta, label_smoothing)
+
+
+def _pack_preference(tensors, rest) -> bytes:
+    x, ref, mask, y, y_ref, y_mask = tensors
+    return L.PREFERENCE_LOSS.pack(*_plane(x), *_plane(ref), *_plane(mask), x.shape[1], *_plane(y), *_plane(y_ref), *_plane(y_mask), y.shape[1], *rest)
 
 
 def _pointer(grad, out):
@@ -282,10 +292,11 @@ class _PreferenceLoss(torch.autograd.Function):
     """Loss and the pairs' slopes now; the backward pass spreads the slopes over the valid entries, reading nothing but the masks."""
 
     @staticmethod
-    def forward(ctx, chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, packed):
+    def forward(ctx, chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, rest):
+        packed = _pack_preference((chosen, ref_chosen, chosen_mask, rejected, ref_rejected, rejected_mask), rest)
         out, _, _ = _preference_forward(packed, chosen, rejected, False)
         ctx.save_for_backward(out, chosen_mask, rejected_mask)
-        ctx.packed, ctx.shapes, ctx.dtype = packed, (chosen.shape, rejected.shape), chosen.dtype
+        ctx.rest, ctx.shapes, ctx.dtype = rest, (chosen.shape, rejected.shape), chosen.dtype
         ctx.mark_non_differentiable(out)
         ctx.set_materialize_grads(False)
         return out[0], out
@@ -295,10 +306,13 @@ class _PreferenceLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, _):
         if grad_loss is None:
             return None, None, None, None, None, None, None
-        out = ctx.saved_tensors[0]
+        out, chosen_mask, rejected_mask = ctx.saved_tensors
         gc, gr = (torch.empty(s, device=out.device, dtype=ctx.dtype) for s in ctx.shapes)
         scale = grad_loss.float()
-        L.call("sdeh_preference_grad", out.device, ctx.packed, out.data_ptr(), scale.data_ptr(), 1.0, _pointer(gc, out), _pointer(gr, out))
+        # (the log-probabilities are not read again: the gradients stand in their places)
+        packed = L.PREFERENCE_LOSS.pack(_pointer(gc, out), 0, 0, 0, 0, 0, *_plane(chosen_mask), gc.shape[1], _pointer(gr, out), 0, 0, 0, 0, 0,
+                                        *_plane(rejected_mask), gr.shape[1], *ctx.rest)
+        L.call("sdeh_preference_grad", out.device, packed, out.data_ptr(), scale.data_ptr(), 1.0, _pointer(gc, out), _pointer(gr, out))
         return gc, gr, None, None, None, None, None
 
 
@@ -317,11 +331,11 @@ def preference_loss(chosen: torch.Tensor, rejected: torch.Tensor, ref_chosen: to
     ref_chosen, ref_rejected  like them; None: they are log-ratios already (step_log_ratio)
     *_mask                    bool (or uint8), broadcastable; entries they leave out do not count, whatever they hold
     info                      accuracy (share of the pairs with h > 0), chosen_rewards and rejected_rewards (beta s, [pairs])"""
-    packed, keep = _describe_preference(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, label_smoothing, kind, average)
+    keep, rest = _describe_preference(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, label_smoothing, kind, average)
     if torch.is_grad_enabled() and (chosen.requires_grad or rejected.requires_grad):
-        loss, out = _PreferenceLoss.apply(chosen, rejected, _constant(keep[1]), _constant(keep[4]), keep[2], keep[5], packed)
+        loss, out = _PreferenceLoss.apply(chosen, rejected, _constant(keep[1]), _constant(keep[4]), keep[2], keep[5], rest)
     else:
-        out, _, _ = _preference_forward(packed, chosen, rejected, False)
+        out, _, _ = _preference_forward(_pack_preference(keep, rest), chosen, rejected, False)
         loss = out[0]
     return loss, _preference_info(out, chosen.shape[0])
 
@@ -332,6 +346,6 @@ def preference_loss_and_grad(chosen: torch.Tensor, rejected: torch.Tensor, ref_c
                              average: bool = False, grad_scale: float = 1.0) -> tuple[torch.Tensor, dict, torch.Tensor, torch.Tensor]:
     """`preference_loss` and grad_scale times its gradients without an autograd graph: (loss, info, gradient of chosen, gradient of rejected)."""
     chosen, rejected = chosen.detach(), rejected.detach()
-    packed, keep = _describe_preference(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, label_smoothing, kind, average)
-    out, gc, gr = _preference_forward(packed, chosen, rejected, True, grad_scale)
+    keep, rest = _describe_preference(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, label_smoothing, kind, average)
+    out, gc, gr = _preference_forward(_pack_preference(keep, rest), chosen, rejected, True, grad_scale)
     return out[0], _preference_info(out, chosen.shape[0]), gc, gr

@@ -81,7 +81,8 @@ class AdamW(torch.optim.Optimizer):
 
     `lr` may be a one-element fp32 tensor on the parameters' device (a schedule under a captured graph).  A step never synchronises and may be
     captured (utils/graphs.py: GraphedTrainStep).  Parameters are contiguous fp32, bf16 or fp16 tensors on one HIP device; those without a gradient
-    are left alone.  Parameters must not share memory.  A parameter group added later moves the moments: capture again."""
+    are left alone.  Parameters must not share memory.  A parameter group added later moves the moments: capture again.
+    The state's tensors are views of flat buffers: write into them, do not replace them."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, *, state_bits: int = 32,
                  max_grad_norm: float | None = None, seed: int = 0):

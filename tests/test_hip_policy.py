@@ -587,3 +587,36 @@ def test_gradients_are_differentiable_once():
         assert torch.equal(first, again)
         with pytest.raises(RuntimeError):  # (a gradient of the gradient: there is none, and none is made up)
             again.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("how", ["save_on_cpu", "checkpoint"])
+def test_saved_tensors_may_go_away(how):
+    """Saved tensors that were moved to the host, or made anew, in between: the backward pass reads what it is given, not where they were."""
+    import torch.utils.checkpoint as cp
+
+    lp, old, ref, adv, m = _policy_case(64, 300, torch.float32, "random", "rows")
+    m = m.cuda()
+
+    def run(x, away):
+        def loss(x):
+            y = x * 1.0
+            a = P.policy_loss(y, adv.cuda(), old.cuda(), ref.cuda(), m.clone(), kl_coef=0.1, reduction="rows")[0]
+            b = P.preference_loss(y[:32], y[32:], None, None, m[:32].clone(), m[32:].clone())[0]
+            b = b + P.policy_loss(y, adv.cuda(), mask=m[:1].clone().expand(64, -1))[0]  # (a broadcast mask comes back as a whole one)
+            c = P.step_log_ratio(y.view(64, 50, 6), None, old.cuda().view(64, 50, 6), torch.ones(64, device="cuda")).sum()
+            return a + b + 1e-3 * c
+
+        if away == "save_on_cpu":
+            with torch.autograd.graph.save_on_cpu():
+                value = loss(x)
+        else:
+            value = cp.checkpoint(loss, x, use_reentrant=False) if away else loss(x)
+        junk = [torch.full((64, 300), float("nan"), device="cuda") for _ in range(40)]  # (what was freed is written over)
+        value.backward()
+        del junk
+        return value.detach(), x.grad
+
+    want = run(lp.cuda().requires_grad_(), None)
+    got = run(lp.cuda().requires_grad_(), how)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
