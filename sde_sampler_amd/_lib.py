@@ -215,7 +215,7 @@ PROTOTYPES = {
     "sdeh_reduce_estimators": (C.c_int32, [fp, C.c_int64, C.c_float, fp, fp, C.c_void_p]),
     "sdeh_step_log_ratio": (C.c_int32, [fp, fp, fp, fp, C.c_int64, C.c_int64, C.c_int32, C.c_int32, fp, C.c_void_p]),
     "sdeh_step_log_ratio_backward": (C.c_int32, [fp, fp, fp, fp, fp, C.c_int64, C.c_int64, C.c_int32, C.c_int32, fp, C.c_void_p]),
-    "sdeh_policy_loss_scratch_floats": (C.c_int64, [C.c_int64]),
+    "sdeh_policy_loss_scratch_floats": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32]),
     "sdeh_policy_loss": (C.c_int32, [C.c_char_p, fp, C.c_int32, fp, C.c_float, fp, fp, C.c_void_p]),
     "sdeh_preference_loss_scratch_floats": (C.c_int64, [C.c_char_p]),
     "sdeh_preference_loss": (C.c_int32, [C.c_char_p, fp, C.c_float, fp, fp, fp, C.c_void_p]),

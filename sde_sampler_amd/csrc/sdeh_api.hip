@@ -21,7 +21,7 @@ int launch_guard_restore(const unsigned long long* table, int n_tensors, const u
 int launch_guard_check(float* g, long long n, const float* value, float max_loss, unsigned char* ok, hipStream_t stream);
 int launch_step_log_ratio(const void* u, const void* v, const void* dw, const float* dt, const float* g, long long n_steps, long long batch, int dim,
                           int dtype, void* out, hipStream_t stream);                                                        // sdeh_policy.hip
-long long policy_scratch_floats(long long rows);
+long long policy_scratch_floats(long long rows, long long steps, bool masked);
 int launch_policy_loss(const SdehPolicyLoss& p, float* scratch, int reuse_counts, const float* grad_scale, float grad_factor, float* out, void* grad,
                        hipStream_t stream);
 long long preference_scratch_floats(const SdehPreferenceLoss& p);
@@ -2006,7 +2006,9 @@ int32_t sdeh_step_log_ratio_backward(const void* control, const void* behaviour,
   return step_log_ratio("step_log_ratio_backward", control, behaviour, increments, dt, grad, n_steps, batch, dim, dtype, grad_control, true, stream);
 }
 
-int64_t sdeh_policy_loss_scratch_floats(int64_t rows) { return rows < 0 ? 0 : policy_scratch_floats(rows); }
+int64_t sdeh_policy_loss_scratch_floats(int64_t rows, int64_t steps, int32_t masked) {
+  return rows < 0 || steps < 0 || (rows > 0 && steps > INT64_MAX / 16 / rows) ? 0 : policy_scratch_floats(rows, steps, masked != 0);
+}
 
 int32_t sdeh_policy_loss(const SdehPolicyLoss* p, float* scratch, int32_t reuse_counts, const float* grad_scale, float grad_factor, float* out,
                          void* grad, void* stream) {

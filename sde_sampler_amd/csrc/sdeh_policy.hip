@@ -791,7 +791,10 @@ int launch_policy_t(PolicyArgs a, bool reuse_counts, hipStream_t stream) {
 }  // namespace
 
 // scratch: partial sums, partial counts, row counts
-long long policy_scratch_floats(long long rows) { return kPolicyBlocks * 8ll + kCountBlocks * 2ll + (rows + 1) / 2 * 2; }
+long long policy_scratch_floats(long long rows, long long steps, bool masked) {
+  if (!masked && rows * steps <= kPolicySmall) return 0;
+  return kPolicyBlocks * 8ll + kCountBlocks * 2ll + (rows + 1) / 2 * 2;
+}
 
 int launch_policy_loss(const SdehPolicyLoss& p, float* scratch, int reuse_counts, const float* grad_scale, float grad_factor, float* out,
                        void* grad, hipStream_t stream) {

@@ -145,8 +145,10 @@ def _pack_policy(tensors, rest) -> bytes:
     return L.POLICY_LOSS.pack(*_plane(log_prob), *_plane(old), *_plane(ref), *adv, *_plane(mask), *rest)
 
 
-def _policy_scratch(log_prob):
-    return torch.empty(L.load().sdeh_policy_loss_scratch_floats(log_prob.shape[0]), device=log_prob.device, dtype=torch.float32)
+def _policy_scratch(log_prob, mask, out=None):
+    """Scratch of a call; where it needs none, `out` stands for it."""
+    n = L.load().sdeh_policy_loss_scratch_floats(*log_prob.shape, mask is not None)
+    return out if n == 0 and out is not None else torch.empty(max(n, 4), device=log_prob.device, dtype=torch.float32)
 
 
 def _policy_info(out):
@@ -160,7 +162,7 @@ class _PolicyLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, log_prob, advantage, old, ref, mask, rest):
-        scratch = _policy_scratch(log_prob)
+        scratch = _policy_scratch(log_prob, mask)
         out = torch.empty(5, device=log_prob.device, dtype=torch.float32)
         packed = _pack_policy((log_prob, advantage, old, ref, mask), rest)
         L.call("sdeh_policy_loss", log_prob.device, packed, scratch.data_ptr(), 0, None, 1.0, out.data_ptr(), None)
@@ -210,7 +212,7 @@ def policy_loss(log_prob: torch.Tensor, advantage: torch.Tensor, old_log_prob: t
         return loss, _policy_info(out)
     packed = _pack_policy(tensors, rest)
     out = torch.empty(5, device=x.device, dtype=torch.float32)
-    scratch = _policy_scratch(x)
+    scratch = _policy_scratch(x, tensors[4], out)
     L.call("sdeh_policy_loss", x.device, packed, scratch.data_ptr(), 0, None, 1.0, out.data_ptr(), None)
     return out[0], _policy_info(out)
 
@@ -226,7 +228,7 @@ def policy_loss_and_grad(log_prob: torch.Tensor, advantage: torch.Tensor, old_lo
     x, packed = tensors[0], _pack_policy(tensors, rest)
     out = torch.empty(5, device=x.device, dtype=torch.float32)
     grad = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    scratch = _policy_scratch(x)
+    scratch = _policy_scratch(x, tensors[4], out)
     L.call("sdeh_policy_loss", x.device, packed, scratch.data_ptr(), 0, None, grad_scale, out.data_ptr(), grad.data_ptr())
     return out[0], _policy_info(out), grad
 

@@ -7,6 +7,8 @@ import itertools
 
 import numpy as np
 import torch
+from torch.optim.optimizer import _global_optimizer_post_hooks as _global_post
+from torch.optim.optimizer import _global_optimizer_pre_hooks as _global_pre
 
 from sde_sampler_amd import _lib as L
 
@@ -211,6 +213,15 @@ class AdamW(torch.optim.Optimizer):
     def step(self, closure=None, *, ok: torch.Tensor | None = None):
         """One step.  ok: an optional one-element bool tensor on the device; where it is False, parameters, moments and step counters stay as they are
         (the decision of `if loss_ok and grad_ok`, solver/base.py:409-421, without a host round trip), and `grad_norm` too."""
+        if self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _global_pre or _global_post or torch.autograd._profiler_enabled():
+            return self._hooked_step(closure, ok=ok)
+        return self._step(closure, ok=ok)
+
+    #: torch.optim.Optimizer would wrap `step` for its hooks and the profiler, which costs a quarter of a small model's step: `step` goes through that
+    #: wrapper (`_hooked_step`) only when there is a hook or a profiler
+    step.hooked = True
+
+    def _step(self, closure=None, *, ok: torch.Tensor | None = None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -239,3 +250,5 @@ class AdamW(torch.optim.Optimizer):
                             self.seed & 0xFFFFFFFF, len(groups))
         L.call("sdeh_adamw_step", self._device, head, b"".join(groups), table.ctypes.data, self._scratch.data_ptr())
         return loss
+
+    _hooked_step = torch.optim.Optimizer.profile_hook_step(_step)

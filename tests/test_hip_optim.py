@@ -307,6 +307,28 @@ def test_learning_rate_on_the_device_and_closure():
 
 
 @gpu
+def test_step_hooks_and_the_profiler():
+    from torch.optim.optimizer import register_optimizer_step_post_hook
+
+    p = _params([10], torch.float32)
+    opt, seen = AdamW(p), []
+    _set_grads(p, 0)
+    handles = [opt.register_step_pre_hook(lambda *a: seen.append("pre")), opt.register_step_post_hook(lambda *a: seen.append("post"))]
+    opt.step()
+    for h in handles:
+        h.remove()
+    assert seen == ["pre", "post"]
+    h = register_optimizer_step_post_hook(lambda *a: seen.append("all"))
+    opt.step()
+    h.remove()
+    opt.step()
+    assert seen == ["pre", "post", "all"] and float(opt.state[p[0]]["step"]) == 3.0
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        opt.step(ok=torch.ones(1, dtype=torch.bool, device="cuda"))
+    assert any("AdamW.step" in e.key for e in prof.key_averages()) and float(opt.state[p[0]]["step"]) == 4.0
+
+
+@gpu
 def test_second_moment_in_8_bits_decays_as_it_should():
     """2000 steps without gradients: rounding to the nearest would never leave the first code.  A step's rounding moves an entry by a code (at most 1/8)
     with probability at most 0.001 x 16: relative variance below 0.016 / 64 a step, 0.5 in all; the mean of 65536 entries is off by less than
