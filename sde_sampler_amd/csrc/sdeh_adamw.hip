@@ -3,9 +3,11 @@
 // With 32-bit moments bounded by memory: fp32 reads and writes 28 bytes an entry (and the gradient's 4 once more for the norm); 150 M entries take
 // 0.78 ms (5.4 TB/s; a large elementwise kernel reaches 6.2) after 0.12 ms for the norm.  With 8-bit moments it is 10 bytes of bf16 (and 2) but some 65
 // vector instructions an entry -- codes, two hashed roundings, the update --: 100 M entries take 0.21 ms, of which the instructions alone 0.17, and the
-// norm 0.04.  Small models are bounded by two launches, 9 us.  Two launches for each 48 tensors: the first forms partial sums of the gradients' squares and the tensors' coefficients
-// (step counters, bias corrections), the second adds the partial sums up again in every workgroup -- 2048 doubles from L2 -- and updates.  The
-// tensors' pointers travel as kernel arguments: no table on the device, nothing to keep or to invalidate.
+// norm 0.04.  Small models are bounded by two launches, 9 us.
+//
+// Two launches for each 48 tensors: the first forms partial sums of the gradients' squares and the tensors' coefficients (step counters, bias
+// corrections), the second adds the partial sums up again in every workgroup -- up to 2048 doubles from L2 -- and updates.  The tensors' pointers travel as
+// kernel arguments: no table on the device, nothing to keep or to invalidate.
 #include "sdeh_elem.hpp"
 
 namespace sdeh {
