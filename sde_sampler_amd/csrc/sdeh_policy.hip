@@ -1139,11 +1139,11 @@ constexpr long long kPreferenceSmall = 4096;
 constexpr long long kShortRow = 1024;         // rows that a wave sums
 constexpr int kMaxSplits = 64;
 
-// parts of a row: a workgroup a part of 4096 entries or more, and 3072 workgroups where rows are few (those that get padding end at once)
+// parts of a row: a workgroup a part of 4096 entries or more, and 2048 workgroups where rows are few (those that get padding end at once)
 int preference_splits(const SdehPreferenceLoss& p) {
   const long long longest = p.chosen.steps > p.rejected.steps ? p.chosen.steps : p.rejected.steps;
   if (longest <= kShortRow) return 1;
-  long long s = (3072 + 2 * p.pairs - 1) / (2 * p.pairs), most = (longest + 4095) / 4096;
+  long long s = (2048 + 2 * p.pairs - 1) / (2 * p.pairs), most = (longest + 4095) / 4096;
   s = s > most ? most : s;
   return (int)(s > kMaxSplits ? kMaxSplits : s < 1 ? 1 : s);
 }

@@ -292,6 +292,24 @@ def test_ok_decides_on_the_device():
 
 
 @gpu
+def test_past_32_bit_offsets():
+    """More than 2^31 entries in one tensor: its end is updated like its beginning."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 48 << 30:
+        pytest.skip("needs 48 GiB of device memory")
+    n = (1 << 31) + 4099
+    p = torch.nn.Parameter(torch.ones(n, device="cuda", dtype=torch.bfloat16))
+    p.grad = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    spots = [0, 255, (1 << 31) - 1, 1 << 31, (1 << 31) + 257, n - 1]
+    p.grad[spots] = 1.0
+    opt = AdamW([p], lr=0.5, weight_decay=0.0, state_bits=8, max_grad_norm=0.25)
+    opt.step()
+    assert abs(float(opt.grad_norm) - math.sqrt(6)) <= 4 * H
+    p = p.detach()
+    assert int((p != 1.0).sum()) == len(spots) and bool((p[spots] == 0.5).all())  # (a first step moves by lr, whatever the gradient's size)
+
+
+@gpu
 def test_learning_rate_on_the_device_and_closure():
     a, b = _params([500], torch.float32), _params([500], torch.float32)
     lr = torch.tensor(0.01, device="cuda")

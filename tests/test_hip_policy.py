@@ -620,3 +620,66 @@ def test_saved_tensors_may_go_away(how):
     want = run(lp.cuda().requires_grad_(), None)
     got = run(lp.cuda().requires_grad_(), how)
     assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+BIG = (1 << 31) + 4099  # elements, odd
+
+
+def _room(gib):
+    free, _ = torch.cuda.mem_get_info()
+    if free < gib << 30:
+        pytest.skip(f"needs {gib} GiB of device memory")
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 3])
+def test_policy_loss_past_32_bit_offsets(rows):
+    """More than 2^31 entries: what lies behind them is read and written where it is.  All entries alike but the last few and one at 2^31."""
+    _room(24)
+    T = -(-BIG // rows)
+    if rows == 1:
+        T = (1 << 31) - 1  # the most steps a row may have; the second row's entries lie past 2^31
+        rows = 2
+    x = torch.full((rows, T), -0.125, device="cuda", dtype=torch.bfloat16)
+    spots = [(0, 0), (rows - 1, T - 1), (rows - 1, T - 700), (rows - 1, 5)]
+    for k, (r, c) in enumerate(spots):
+        x[r, c] = 0.25 + 0.125 * k  # beyond the upper border
+    mask = torch.ones(rows, T, device="cuda", dtype=torch.bool)
+    mask[rows - 1, T - 2] = False
+    loss, info, grad = P.policy_loss_and_grad(x, torch.ones(rows, device="cuda"), mask=mask, reduction="sum")
+    n = rows * T - 1
+    want = -((n - 4) * math.exp(-0.125) + 4 * 1.2)
+    assert abs(float(loss) - want) <= 12 * H * abs(want)
+    assert float(info["clip_fraction"]) == pytest.approx(4 / n, rel=1e-6)
+    assert all(float(grad[s]) == 0.0 for s in spots) and float(grad[rows - 1, T - 2]) == 0.0
+    flat = grad.view(-1)
+    usual = float(torch.tensor(-math.exp(-0.125)).bfloat16())
+    assert int((flat[-1000:] == usual).sum()) == 1000 - 3 and int((flat != usual).sum()) == 5
+
+
+@gpu
+def test_preference_loss_past_32_bit_offsets():
+    _room(24)
+    x = torch.zeros(1, BIG, device="cuda", dtype=torch.bfloat16)
+    y = torch.zeros(1, 3, device="cuda", dtype=torch.bfloat16)
+    x[0, -1], x[0, 1 << 31] = 2.0, 3.0
+    loss, info, gx, gy = P.preference_loss_and_grad(x, y, beta=1.0)
+    assert float(info["chosen_rewards"]) == 5.0 and abs(float(loss) - math.log1p(math.exp(-5.0))) < 1e-8
+    assert bool((gx == gx[0, 0]).all()) and float(gx[0, 0]) == -float(gy[0, 0]) != 0.0
+
+
+@gpu
+def test_step_log_ratio_past_32_bit_offsets():
+    _room(48)
+    T, d = 3, 7
+    B = -(-BIG // (T * d))
+    u = torch.zeros(T, B, d, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    dw = torch.full((T, B, d), 0.5, device="cuda", dtype=torch.bfloat16)
+    dt = torch.tensor([0.1, 0.2, 0.5], device="cuda")
+    with torch.no_grad():
+        u[-1, -1], u[-1, -2, 0] = 2.0, 1.0
+    y = P.step_log_ratio(u, None, dw, dt)
+    y.backward(torch.ones_like(y))
+    y = y.detach()
+    assert float(y[-1, -1]) == 7 * (2.0 * 0.5 - 0.25 * 4.0) and float(y[-1, -2]) == 0.25 and int((y != 0).sum()) == 1
+    assert bool((u.grad[-1, -1] == -0.5).all()) and float(u.grad[-1, -2, 0]) == 0.0 and int((u.grad != 0.5).sum()) == 8
