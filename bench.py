@@ -174,7 +174,9 @@ def cpu_process_parallel(spec, prob_cpu_state, chunk: int, n_intervals: int | No
     import subprocess
     import tempfile
 
-    n = int(os.environ.get("SDEH_BENCH_CPU_PROCS", usable_cpus()))  # (round 5: the cores this container may use, not the host's 128)
+    # the cores this container may use, not the host's 128; 14 at most: an interpreter with torch loaded opens the GPU's device file although no GPU is
+    # visible to it, and a host may allow 16 such processes, this one among them
+    n = int(os.environ.get("SDEH_BENCH_CPU_PROCS", min(usable_cpus(), 14)))
     try:  # an interpreter with torch loaded is ~0.5 GB resident: never more processes than the host's free memory holds three times over
         import psutil
 
