@@ -422,6 +422,13 @@ def test_loads_torch_state_and_refuses_other_formats():
     theirs.step()
     for x, y in zip(a, b):
         torch.testing.assert_close(x, y, rtol=8 * H, atol=1e-2 * 40 * H)
+    assert "capturable" not in ours.param_groups[0]
+    back = torch.optim.AdamW(b, lr=1.0)
+    back.load_state_dict(ours.state_dict())
+    assert back.param_groups[0]["lr"] == 1e-2 and torch.equal(back.state[b[0]]["exp_avg"], ours.state[a[0]]["exp_avg"])
+    for other in (torch.optim.AdamW(b, amsgrad=True), torch.optim.AdamW(b, maximize=True), torch.optim.Adam(b, weight_decay=0.1)):
+        with pytest.raises(ValueError, match="amsgrad"):
+            ours.load_state_dict(other.state_dict())
     with pytest.raises(ValueError, match="state_bits"):
         AdamW(_params([50, 4], torch.float32), state_bits=8).load_state_dict(ours.state_dict())
     with pytest.raises(ValueError):
