@@ -167,10 +167,11 @@ __global__ __launch_bounds__(kThreads) void ratio_forward_kernel(RatioArgs a, un
       for (int k = 0; k < V; ++k) {
         const float e = keep != 0.0f ? pu[k] - pv[k] : pu[k];
         const bool here = k < left;
-        s1 = fmaf(here ? e : 0.0f, pw[k], s1);
-        s2 = fmaf(here ? e : 0.0f, e, s2);
-        a1 = fmaf(here ? 0.0f : e, pw[k], a1);
-        a2 = fmaf(here ? 0.0f : e, e, a2);
+        const float eh = here ? e : 0.0f, ea = here ? 0.0f : e;  // (both factors: 0 times an infinite neighbour would be NaN in this row)
+        s1 = fmaf(eh, here ? pw[k] : 0.0f, s1);
+        s2 = fmaf(eh, eh, s2);
+        a1 = fmaf(ea, here ? 0.0f : pw[k], a1);
+        a2 = fmaf(ea, ea, a2);
       }
       before[i] = fmaf(-row_dt[r], s2, s1);
       after[i] = left < V ? fmaf(-row_dt[r + 1], a2, a1) : 0.0f;

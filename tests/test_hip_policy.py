@@ -110,6 +110,36 @@ def test_step_log_ratio_gradient_against_differences():
         assert abs(float(d - ug.grad.view(-1)[i])) <= 40 * H * (size + 1) / step
 
 
+@gpu
+@pytest.mark.parametrize("d", [1, 3, 5, 6, 10, 50, 196, 513])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("where", ["control", "behaviour", "increments"])
+def test_step_log_ratio_keeps_trajectories_apart(d, dtype, where):
+    """A trajectory that diverged -- one NaN or infinite coordinate, at a row's first, last or middle place -- has no finite ratio at that step; every other
+    ratio and gradient is what it is without it, bit for bit, aligned or not."""
+    T, B = 4, 23
+    u, v, dw, dt, g = _ratio_case(T, B, d, dtype)
+    off = lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)]).cuda()[1:].view(t.shape)  # noqa: E731
+    for place in (lambda t: t.cuda(), off):
+        clean_u = place(u).detach().requires_grad_()
+        clean = P.step_log_ratio(clean_u, place(v), place(dw), dt.cuda())
+        clean.backward(g.cuda())
+        for bad in (math.nan, math.inf, -math.inf):
+            case = {"control": u.clone(), "behaviour": v.clone(), "increments": dw.clone()}
+            spots = {(0, 0): 0, (1, 7): d - 1, (2, 8): 0, (2, 12): d // 2, (T - 1, B - 1): d - 1}
+            for (t, b), k in spots.items():
+                case[where][t, b, k] = bad
+            x = place(case["control"]).detach().requires_grad_()
+            y = P.step_log_ratio(x, place(case["behaviour"]), place(case["increments"]), dt.cuda())
+            y.backward(g.cuda())
+            hit = torch.zeros(T, B, dtype=torch.bool)
+            for t, b in spots:
+                hit[t, b] = True
+            y, want = y.detach().cpu(), clean.detach().cpu()
+            assert torch.equal(~torch.isfinite(y), hit)
+            assert torch.equal(y[~hit], want[~hit]) and torch.equal(x.grad.cpu()[~hit], clean_u.grad.cpu()[~hit])
+
+
 # -- policy loss ---------------------------------------------------------------------------------------------------------------------------
 def _policy_case(R, T, dtype, mask="ragged", adv="rows", ref=True, seed=0):
     g = torch.Generator().manual_seed(seed + 13 * R + T)
