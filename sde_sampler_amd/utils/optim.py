@@ -46,7 +46,7 @@ class _Bucket:
             self.table[i, 2:] = (s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(), *top, s["step"].data_ptr(), size, first_block + b0)
 
     def rows(self):
-        """(the table's rows of the parameters that have a gradient, the gradients, kept alive)"""
+        """(the table's rows of the parameters that have a gradient, the gradients, kept alive, and the tensors that a step on these rows writes)"""
         index, dtype = self.device.index, self.dtype
         param, grad, keep, missing = [], [], [], False
         for p, n in zip(self.params, self.sizes):
@@ -68,7 +68,9 @@ class _Bucket:
             grad.append(g.data_ptr())
         self.table[:, 0] = param
         self.table[:, 1] = grad
-        return (self.table[self.table[:, 0] != 0] if missing else self.table), keep
+        if not missing:
+            return self.table, keep, [*self.params, *self.flat.values()]
+        return self.table[self.table[:, 0] != 0], keep, [*(p for p in self.params if p.grad is not None), *self.flat.values()]
 
 
 class AdamW(torch.optim.Optimizer):
@@ -232,7 +234,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        groups, tables, keep = [], [], []
+        groups, tables, keep, written = [], [], [], []
         for group, buckets in self._plan():
             lr, (b1, b2) = group["lr"], group["betas"]
             lr_dev = 0
@@ -241,11 +243,12 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("AdamW: a tensor lr must be one fp32 element on the parameters' device")
                 lr, lr_dev = 0.0, lr.data_ptr()
             for b in buckets:
-                rows, held = b.rows()
+                rows, held, tensors = b.rows()
                 if len(rows):
                     groups.append(L.ADAMW_GROUP.pack(lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, len(rows), b.code, b.bits, 0))
                     tables.append(rows)
                     keep.append(held)
+                    written += tensors
         if not groups:
             return loss
         if ok is not None and (ok.device != self._device or ok.numel() != 1 or ok.dtype not in (torch.bool, torch.uint8)):
@@ -255,6 +258,11 @@ class AdamW(torch.optim.Optimizer):
         head = L.ADAMW.pack(self.max_grad_norm or 0.0, 0 if ok is None else ok.data_ptr(), 0 if norm is None else norm.data_ptr(),
                             self.seed & 0xFFFFFFFF, len(groups))
         L.call("sdeh_adamw_step", self._device, head, b"".join(groups), table.ctypes.data, self._scratch.data_ptr())
+        if norm is not None:
+            written.append(norm)
+        # (written behind torch's back: whoever saved one of them for a backward pass, or cached what it held, is told here -- also where `ok` is False,
+        # which the host does not know)
+        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
         return loss
 
     _hooked_step = torch.optim.Optimizer.profile_hook_step(_step)

@@ -363,6 +363,27 @@ def test_second_moment_in_8_bits_decays_as_it_should():
     assert abs(float(opt.moments()[1].mean(dtype=torch.float64)) - want) <= want * 6 * math.sqrt(0.5 / 65536)
 
 
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_is_seen_by_autograd(bits):
+    """As with torch's optimizers: a graph whose forward pass saved a parameter before the step refuses its backward pass after it."""
+    for make in (lambda ps: torch.optim.AdamW(ps), lambda ps: AdamW(ps, state_bits=bits, max_grad_norm=1.0)):
+        p, idle = _params([12, 5], torch.float32)
+        opt = make([p, idle])
+        p.grad = torch.ones_like(p)
+        opt.step()
+        loss = (p * p).sum()
+        versions = p._version, idle._version
+        opt.step()
+        assert p._version > versions[0] and idle._version == versions[1]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    version = p._version
+    norm = opt.grad_norm._version
+    opt.step(ok=torch.ones(1, dtype=torch.bool, device="cuda"))
+    assert p._version > version and opt.grad_norm._version > norm
+
+
 # -- state dicts ------------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
