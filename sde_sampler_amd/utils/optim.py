@@ -173,14 +173,21 @@ class AdamW(torch.optim.Optimizer):
             t.copy_(s.reshape(t.shape))
 
     def load_state_dict(self, state_dict):
-        """Values are copied into this optimizer's own buffers: a captured step keeps working on them.  A state dict of torch.optim.AdamW (or Adam, without
+        """Values are copied into this optimizer's own buffers, learning rates on the device into their own tensors: a captured step keeps working on them.  A state dict of torch.optim.AdamW (or Adam, without
         weight decay) fits 32-bit moments; its flags about how to compute are dropped, those about what (amsgrad, maximize) are refused."""
         for group in state_dict["param_groups"]:
             if group.get("amsgrad") or group.get("maximize") or (group["weight_decay"] and group.get("decoupled_weight_decay") is False):
                 raise ValueError("AdamW: a state dict with amsgrad, maximize or coupled weight decay")
         buckets, norm = self._buckets, self.grad_norm
+        rates = [group["lr"] for group in self.param_groups]
         super().load_state_dict({**state_dict, "state": {}})  # groups and their hyperparameters (the base class would cast moments to the parameters' type)
-        for group in self.param_groups:
+        for group, rate in zip(self.param_groups, rates):
+            if isinstance(rate, torch.Tensor):
+                with torch.no_grad():
+                    rate.copy_(torch.as_tensor(group["lr"]).reshape(rate.shape))
+                group["lr"] = rate
+            elif isinstance(group["lr"], torch.Tensor):  # (from wherever it was loaded to)
+                group["lr"] = group["lr"].to(group["params"][0].device, torch.float32)
             for key in ("amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay"):
                 group.pop(key, None)
             self._check_group(group)

@@ -460,6 +460,51 @@ def test_loads_torch_state_and_refuses_other_formats():
     assert torch.equal(ours.state[a[0]]["exp_avg"], kept)
 
 
+@gpu
+def test_loading_keeps_the_learning_rate_on_the_device():
+    """`lr` on the device stays the tensor that the caller and a captured step hold; what is loaded -- from the device, the host or a number -- is its value."""
+    p, q = _params([40], torch.float32), _params([40], torch.float32)
+    lr = torch.tensor(0.5, device="cuda")
+    opt = AdamW(p, lr=lr, weight_decay=0.0)
+    _set_grads(p, 0)
+    opt.step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step()
+    saved = copy.deepcopy(opt.state_dict())  # (a state dict refers to the optimizer's own tensors)
+    buf = io.BytesIO()
+    torch.save(saved, buf)
+    other = AdamW(q, lr=0.25, weight_decay=0.0)
+    for state, value in ((saved, 0.5), (torch.load(io.BytesIO(buf.getvalue()), map_location="cpu", weights_only=True), 0.5), (other.state_dict(), 0.25)):
+        lr.fill_(9.0)
+        opt.load_state_dict(state)
+        assert opt.param_groups[0]["lr"] is lr and float(lr) == value
+    other.load_state_dict(opt.state_dict())
+    with torch.no_grad():
+        q[0].copy_(p[0])
+    q[0].grad = p[0].grad.clone()
+    lr.fill_(0.125)
+    other.param_groups[0]["lr"] = 0.125
+    g.replay()
+    other.step()
+    assert torch.equal(p[0], q[0])
+
+
+@gpu
+def test_a_state_dict_with_its_rate_on_the_host():
+    a, b = _params([40], torch.float32), _params([40], torch.float32)
+    opt = AdamW(a, lr=torch.tensor(0.5, device="cuda"))
+    _set_grads(a, 0)
+    opt.step()
+    saved = opt.state_dict()
+    saved["param_groups"][0]["lr"] = saved["param_groups"][0]["lr"].cpu()
+    other = AdamW(b, lr=0.1)
+    other.load_state_dict(saved)
+    _set_grads(b, 0)
+    other.step()
+    assert float(other.param_groups[0]["lr"]) == 0.5 and float(other.state[b[0]]["step"]) == 2.0
+
+
 # -- graphs, streams ----------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
