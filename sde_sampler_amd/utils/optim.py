@@ -180,7 +180,31 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("AdamW: a state dict with amsgrad, maximize or coupled weight decay")
         buckets, norm = self._buckets, self.grad_norm
         rates = [group["lr"] for group in self.param_groups]
-        super().load_state_dict({**state_dict, "state": {}})  # groups and their hyperparameters (the base class would cast moments to the parameters' type)
+        loaded = {}
+
+        # The base class loads groups and their hyperparameters; moments it would cast to the parameters' type.  They are taken out behind the last of the
+        # caller's pre-hooks and put in before the first of its post-hooks.
+        def take_out(_, state_dict):
+            loaded.update(state_dict)
+            return {**state_dict, "state": {}}
+
+        def put_in(_):
+            self._take_groups(rates)
+            if buckets is not None:  # (the same parameters in the same groups: only the groups' dicts are new)
+                self._buckets, self.grad_norm = [(group, bs) for group, (_, bs) in zip(self.param_groups, buckets)], norm
+            saved = itertools.chain.from_iterable(g["params"] for g in loaded["param_groups"])
+            params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
+            self._take_state({p: loaded["state"].get(i) for i, p in zip(saved, params)})
+
+        hooks = self.register_load_state_dict_pre_hook(take_out), self.register_load_state_dict_post_hook(put_in, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _take_groups(self, rates) -> None:
+        """Groups as they were loaded; `rates`: the learning rates before."""
         for group, rate in zip(self.param_groups, rates):
             if isinstance(rate, torch.Tensor):
                 with torch.no_grad():
@@ -191,11 +215,8 @@ class AdamW(torch.optim.Optimizer):
             for key in ("amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay"):
                 group.pop(key, None)
             self._check_group(group)
-        saved = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
-        params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
-        entries = {p: state_dict["state"].get(i) for i, p in zip(saved, params)}
-        if buckets is not None:  # (the same parameters in the same groups: only the groups' dicts are new)
-            self._buckets, self.grad_norm = [(group, bs) for group, (_, bs) in zip(self.param_groups, buckets)], norm
+
+    def _take_state(self, entries: dict) -> None:
         for _, buckets in self._plan():
             for b in buckets:
                 for p, own in zip(b.params, b.states):

@@ -505,6 +505,26 @@ def test_a_state_dict_with_its_rate_on_the_host():
     assert float(other.param_groups[0]["lr"]) == 0.5 and float(other.state[b[0]]["step"]) == 2.0
 
 
+@gpu
+def test_load_hooks_see_and_change_the_state():
+    """A pre-hook is given the whole state dict and may change it; a post-hook finds the state loaded."""
+    params = _params([8], torch.float32)
+    opt, seen = AdamW(params), []
+    _set_grads(params, 0)
+    opt.step()
+    saved = opt.state_dict()
+    moments = saved["state"][0]["exp_avg"].clone()
+
+    def double(o, s):
+        seen.append(len(s["state"]))
+        return {**s, "state": {0: {**s["state"][0], "exp_avg": 2 * moments}}}
+
+    opt.register_load_state_dict_pre_hook(double)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append(o.state[params[0]]["exp_avg"].clone()))
+    opt.load_state_dict(saved)
+    assert seen[0] == 1 and torch.equal(seen[1], 2 * moments)
+
+
 # -- graphs, streams ----------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
