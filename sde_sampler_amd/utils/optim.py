@@ -163,35 +163,55 @@ class AdamW(torch.optim.Optimizer):
         return plan
 
     @staticmethod
-    def _adopt(own: dict, other: dict) -> None:
+    def _check_state(own: dict, other: dict) -> None:
         if set(other) != set(own):
             raise ValueError(f"AdamW: a state with {sorted(other)} does not fit one with {sorted(own)} (state_bits differ?)")
         for k, t in own.items():
             s = torch.as_tensor(other[k])
             if s.numel() != t.numel() or (t.dtype == torch.uint8) != (s.dtype == torch.uint8):
                 raise ValueError(f"AdamW: {k} is {tuple(s.shape)} {s.dtype}, expected {tuple(t.shape)} {t.dtype}")
-            t.copy_(s.reshape(t.shape))
+
+    def _adopt(self, own: dict, other: dict) -> None:
+        self._check_state(own, other)
+        for k, t in own.items():
+            t.copy_(torch.as_tensor(other[k]).reshape(t.shape))
+
+    def _check_loaded(self, state_dict) -> None:
+        """Refuses what does not fit, before anything is changed.  (Numbers of groups and parameters are the base class's to refuse.)"""
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize") or (group.get("weight_decay") and group.get("decoupled_weight_decay") is False):
+                raise ValueError("AdamW: a state dict with amsgrad, maximize or coupled weight decay")
+            lacks = [k for k in ("lr", "betas", "eps", "weight_decay") if k not in group]
+            if lacks:
+                raise ValueError(f"AdamW: a state dict whose groups lack {lacks}")
+            lr = group["lr"]
+            if isinstance(lr, torch.Tensor) and lr.numel() != 1:
+                raise ValueError(f"AdamW: a tensor lr must be one element, got {tuple(lr.shape)}")
+            self._check_group({**group, "lr": 0.0} if isinstance(lr, torch.Tensor) else group)
+        states = {id(p): own for _, buckets in self._plan() for b in buckets for p, own in zip(b.params, b.states)}
+        for ours, theirs in zip(self.param_groups, state_dict["param_groups"]):
+            for p, i in zip(ours["params"], theirs["params"]):
+                if state_dict["state"].get(i):
+                    self._check_state(states[id(p)], state_dict["state"][i])
 
     def load_state_dict(self, state_dict):
-        """Values are copied into this optimizer's own buffers, learning rates on the device into their own tensors: a captured step keeps working on them.  A state dict of torch.optim.AdamW (or Adam, without
-        weight decay) fits 32-bit moments; its flags about how to compute are dropped, those about what (amsgrad, maximize) are refused."""
-        for group in state_dict["param_groups"]:
-            if group.get("amsgrad") or group.get("maximize") or (group["weight_decay"] and group.get("decoupled_weight_decay") is False):
-                raise ValueError("AdamW: a state dict with amsgrad, maximize or coupled weight decay")
-        buckets, norm = self._buckets, self.grad_norm
-        rates = [group["lr"] for group in self.param_groups]
-        loaded = {}
+        """Values are copied into this optimizer's own buffers, learning rates on the device into their own tensors: a captured step keeps working on them.
+        A state dict of torch.optim.AdamW (or Adam, without weight decay) fits 32-bit moments; its flags about how to compute are dropped, those about what
+        (amsgrad, maximize) are refused.  A state dict that is refused leaves everything as it was."""
+        loaded, held = {}, {}
 
         # The base class loads groups and their hyperparameters; moments it would cast to the parameters' type.  They are taken out behind the last of the
         # caller's pre-hooks and put in before the first of its post-hooks.
         def take_out(_, state_dict):
+            self._check_loaded(state_dict)
             loaded.update(state_dict)
+            held.update(buckets=[buckets for _, buckets in self._plan()], norm=self.grad_norm, rates=[group["lr"] for group in self.param_groups])
             return {**state_dict, "state": {}}
 
         def put_in(_):
-            self._take_groups(rates)
-            if buckets is not None:  # (the same parameters in the same groups: only the groups' dicts are new)
-                self._buckets, self.grad_norm = [(group, bs) for group, (_, bs) in zip(self.param_groups, buckets)], norm
+            self._take_groups(held["rates"])
+            # (the same parameters in the same groups: only the groups' dicts are new)
+            self._buckets, self.grad_norm = list(zip(self.param_groups, held["buckets"])), held["norm"]
             saved = itertools.chain.from_iterable(g["params"] for g in loaded["param_groups"])
             params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
             self._take_state({p: loaded["state"].get(i) for i, p in zip(saved, params)})
@@ -214,7 +234,6 @@ class AdamW(torch.optim.Optimizer):
                 group["lr"] = group["lr"].to(group["params"][0].device, torch.float32)
             for key in ("amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay"):
                 group.pop(key, None)
-            self._check_group(group)
 
     def _take_state(self, entries: dict) -> None:
         for _, buckets in self._plan():

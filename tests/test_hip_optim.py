@@ -525,6 +525,43 @@ def test_load_hooks_see_and_change_the_state():
     assert seen[0] == 1 and torch.equal(seen[1], 2 * moments)
 
 
+def _all(opt, params):
+    return [t.detach().cpu().clone() for p in params for t in (p, *opt.state[p].values())]
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_load_changes_nothing(bits):
+    params = _params([700, 33], torch.float32)
+    opt = AdamW([{"params": params[:1]}, {"params": params[1:], "lr": 0.5}], state_bits=bits, max_grad_norm=1.0)
+    for k in range(2):
+        _set_grads(params, k)
+        opt.step()
+    before, where = _all(opt, params), [t.data_ptr() for p in params for t in opt.state[p].values()]
+    groups = copy.deepcopy([{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups])
+
+    def broken():
+        for change in (lambda s: s["state"][1].pop("exp_avg"), lambda s: s["state"][1].update(exp_avg=torch.zeros(5)),
+                       lambda s: s["state"][1].update(more=torch.zeros(33)), lambda s: s["param_groups"][1].update(lr=-1.0),
+                       lambda s: s["param_groups"][1].update(betas=(0.9, 1.0)), lambda s: s["param_groups"][1].update(amsgrad=True),
+                       lambda s: s["param_groups"][1].pop("eps"),
+                       lambda s: s["param_groups"].pop(), lambda s: s["param_groups"][1]["params"].append(2)):
+            s = copy.deepcopy(opt.state_dict())
+            s["state"][0]["step"] += 5
+            s["param_groups"][0]["lr"] = 7.0
+            change(s)
+            yield s
+
+    for s in broken():
+        with pytest.raises(ValueError):
+            opt.load_state_dict(s)
+        assert [{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups] == groups
+        assert all(torch.equal(x, y) for x, y in zip(_all(opt, params), before))
+        assert where == [t.data_ptr() for p in params for t in opt.state[p].values()] and opt.grad_norm is not None
+    opt.step()
+    assert float(opt.state[params[0]]["step"]) == 3.0
+
+
 # -- graphs, streams ----------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
