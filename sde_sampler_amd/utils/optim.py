@@ -83,9 +83,9 @@ class AdamW(torch.optim.Optimizer):
                    before clipping (0-d tensor).  The `.grad`s themselves stay as they are
     seed           of the rounding of 8-bit moments
 
-    `lr` may be a one-element fp32 tensor on the parameters' device (a schedule under a captured graph).  A step never synchronises and may be
-    captured (utils/graphs.py: GraphedTrainStep).  Parameters are contiguous fp32, bf16 or fp16 tensors on one HIP device; those without a gradient
-    are left alone.  Parameters must not share memory.  A parameter group added later moves the moments: capture again.
+    `lr` may be a one-element fp32 tensor on the parameters' device (a schedule under a captured graph).  A step never synchronises and, from the second
+    on, may be captured (utils/graphs.py: GraphedTrainStep).  Parameters are contiguous fp32, bf16 or fp16 tensors on one HIP device; those without a
+    gradient are left alone.  Parameters must not share memory.  A parameter group added later moves the moments: step once, then capture again.
     The state's tensors are views of flat buffers: write into them, do not replace them."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, *, state_bits: int = 32,
@@ -129,6 +129,8 @@ class AdamW(torch.optim.Optimizer):
         """[(group, its buckets)]; flat state buffers are made here and take over what `self.state` holds."""
         if self._buckets is not None:
             return self._buckets
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: the state cannot be made while the stream is capturing (every replay would zero it): step once before")
         plan, first, device, seen = [], 0, None, set()
         for group in self.param_groups:
             by_type: dict = {}

@@ -591,6 +591,27 @@ def test_captured_step_replays_the_eager_one(bits):
         assert all(torch.equal(p, q) for p, q in zip(params, twin)) and torch.equal(opt.grad_norm, eager.grad_norm)
 
 
+@gpu
+def test_a_first_step_inside_a_capture_is_refused():
+    """The state's zeros would be part of the graph."""
+    params = _params([50], torch.float32)
+    opt = AdamW(params)
+    _set_grads(params, 0)
+    spare = torch.zeros(4, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        spare += 1
+        with pytest.raises(RuntimeError, match="captur"):
+            opt.step()
+    opt.step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step()
+    for _ in range(3):
+        g.replay()
+    assert float(opt.state[params[0]]["step"]) == 4.0
+
+
 def _problem(seed=0):
     spec = problems.baseline_spec("cfg1_dw_dis_lv")
     torch.manual_seed(seed)
