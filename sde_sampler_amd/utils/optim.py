@@ -129,8 +129,6 @@ class AdamW(torch.optim.Optimizer):
         """[(group, its buckets)]; flat state buffers are made here and take over what `self.state` holds."""
         if self._buckets is not None:
             return self._buckets
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW: the state cannot be made while the stream is capturing (every replay would zero it): step once before")
         plan, first, device, seen = [], 0, None, set()
         for group in self.param_groups:
             by_type: dict = {}
@@ -146,6 +144,8 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("AdamW: a parameter is there twice")
                 seen.add(id(p))
                 by_type.setdefault(p.dtype, []).append(p)
+            if by_type and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: the state cannot be made while the stream is capturing (every replay would zero it): step once before")
             buckets = []
             for params in by_type.values():
                 bucket = _Bucket(params, self.state_bits, first)
