@@ -81,7 +81,7 @@ class AdamW(torch.optim.Optimizer):
                    stochastically, with bits that follow from (seed, step, place): a run is reproducible, and a slow average still moves.
     max_grad_norm  clip the gradients of all groups together to this norm first (clip_grad_norm_'s formula); `grad_norm` then holds their norm
                    before clipping (0-d tensor).  The `.grad`s themselves stay as they are
-    seed           of the rounding of 8-bit moments
+    seed           of the rounding of 8-bit moments (it belongs to the state dict)
 
     `lr` may be a one-element fp32 tensor on the parameters' device (a schedule under a captured graph).  A step never synchronises and, from the second
     on, may be captured (utils/graphs.py: GraphedTrainStep).  Parameters are contiguous fp32, bf16 or fp16 tensors on one HIP device; those without a
@@ -196,6 +196,13 @@ class AdamW(torch.optim.Optimizer):
                 if state_dict["state"].get(i):
                     self._check_state(states[id(p)], state_dict["state"][i])
 
+    def state_dict(self):
+        """As torch.optim.AdamW's; with 8-bit moments also the seed of their rounding, so that a resumed run rounds as the one it goes on with."""
+        out = super().state_dict()
+        if self.state_bits == 8:
+            out["seed"] = self.seed
+        return out
+
     def load_state_dict(self, state_dict):
         """Values are copied into this optimizer's own buffers, learning rates on the device into their own tensors: a captured step keeps working on them.
         A state dict of torch.optim.AdamW (or Adam, without weight decay) fits 32-bit moments; its flags about how to compute are dropped, those about what
@@ -211,6 +218,7 @@ class AdamW(torch.optim.Optimizer):
             return {**state_dict, "state": {}}
 
         def put_in(_):
+            self.seed = int(loaded.get("seed", self.seed))
             self._take_groups(held["rates"])
             # (the same parameters in the same groups: only the groups' dicts are new)
             self._buckets, self.grad_norm = list(zip(self.param_groups, held["buckets"])), held["norm"]

@@ -562,6 +562,24 @@ def test_a_refused_load_changes_nothing(bits):
     assert float(opt.state[params[0]]["step"]) == 3.0
 
 
+@gpu
+def test_the_seed_travels_with_the_state():
+    a, b = _params([3000], torch.float32), _params([3000], torch.float32)
+    x, y = AdamW(a, state_bits=8, seed=5), AdamW(b, state_bits=8)
+    for k in range(2):
+        _set_grads(a, k)
+        x.step()
+    y.load_state_dict(x.state_dict())
+    with torch.no_grad():
+        b[0].copy_(a[0])
+    for k in range(2, 6):
+        _set_grads(a, k)
+        _set_grads(b, k)
+        x.step()
+        y.step()
+    assert torch.equal(a[0], b[0]) and all(torch.equal(x.state[a[0]][k], y.state[b[0]][k]) for k in x.state[a[0]])
+
+
 # -- graphs, streams ----------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
