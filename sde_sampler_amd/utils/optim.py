@@ -98,8 +98,6 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm: torch.Tensor | None = None
         self._buckets: list | None = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
-        for group in self.param_groups:
-            self._check_group(group)
 
     @staticmethod
     def _check_group(group):
@@ -113,8 +111,9 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: betas in [0, 1), eps and weight_decay >= 0, got {group['betas']}, {group['eps']}, {group['weight_decay']}")
 
     def add_param_group(self, param_group):
+        if isinstance(param_group, dict):  # (anything else is the base class's to refuse)
+            self._check_group({**self.defaults, **param_group})
         super().add_param_group(param_group)
-        self._check_group(self.param_groups[-1])
         self._buckets = None
 
     def __getstate__(self):

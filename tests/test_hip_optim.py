@@ -732,6 +732,17 @@ def test_constructor_refuses():
         AdamW(p).step()
 
 
+def test_a_refused_group_is_not_added():
+    p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3))
+    opt = AdamW([p])
+    for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0)):
+        with pytest.raises(ValueError):
+            opt.add_param_group({"params": [q], **bad})
+        assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": [q], "lr": 0.1})
+    assert len(opt.param_groups) == 2
+
+
 def test_c_entry_refuses_bad_arguments():
     lib = L.load()
     head = lambda **k: L.ADAMW.pack(k.get("clip", 1.0), 0, 0, 1, k.get("groups", 1))  # noqa: E731
