@@ -151,6 +151,11 @@ def _policy_scratch(log_prob, mask, out=None):
     return out if n == 0 and out is not None else torch.empty(max(n, 4), device=log_prob.device, dtype=torch.float32)
 
 
+def _loss(out):
+    """out[0] as a tensor of its own, on the same memory: a view of `out` could not be changed in place (`loss /= n`) under autograd."""
+    return out[0].data
+
+
 def _policy_info(out):
     _, policy, kl, fraction, valid = out.unbind()
     return {"policy": policy, "kl": kl, "clip_fraction": fraction, "n_valid": valid}
@@ -170,7 +175,7 @@ class _PolicyLoss(torch.autograd.Function):
         ctx.rest, ctx.mask_stride = rest, None if mask is None else mask.stride()
         ctx.mark_non_differentiable(out)
         ctx.set_materialize_grads(False)  # (no zeros for `out`)
-        return out[0], out
+        return _loss(out), out
 
     @staticmethod
     @_once
@@ -214,7 +219,7 @@ def policy_loss(log_prob: torch.Tensor, advantage: torch.Tensor, old_log_prob: t
     out = torch.empty(5, device=x.device, dtype=torch.float32)
     scratch = _policy_scratch(x, tensors[4], out)
     L.call("sdeh_policy_loss", x.device, packed, scratch.data_ptr(), 0, None, 1.0, out.data_ptr(), None)
-    return out[0], _policy_info(out)
+    return _loss(out), _policy_info(out)
 
 
 def policy_loss_and_grad(log_prob: torch.Tensor, advantage: torch.Tensor, old_log_prob: torch.Tensor | None = None,
@@ -230,7 +235,7 @@ def policy_loss_and_grad(log_prob: torch.Tensor, advantage: torch.Tensor, old_lo
     grad = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     scratch = _policy_scratch(x, tensors[4], out)
     L.call("sdeh_policy_loss", x.device, packed, scratch.data_ptr(), 0, None, grad_scale, out.data_ptr(), grad.data_ptr())
-    return out[0], _policy_info(out), grad
+    return _loss(out), _policy_info(out), grad
 
 
 # -- preference loss -------------------------------------------------------------------------------------------------------------------------
@@ -301,7 +306,7 @@ class _PreferenceLoss(torch.autograd.Function):
         ctx.rest, ctx.shapes, ctx.dtype = rest, (chosen.shape, rejected.shape), chosen.dtype
         ctx.mark_non_differentiable(out)
         ctx.set_materialize_grads(False)
-        return out[0], out
+        return _loss(out), out
 
     @staticmethod
     @_once
@@ -338,7 +343,7 @@ def preference_loss(chosen: torch.Tensor, rejected: torch.Tensor, ref_chosen: to
         loss, out = _PreferenceLoss.apply(chosen, rejected, _constant(keep[1]), _constant(keep[4]), keep[2], keep[5], rest)
     else:
         out, _, _ = _preference_forward(_pack_preference(keep, rest), chosen, rejected, False)
-        loss = out[0]
+        loss = _loss(out)
     return loss, _preference_info(out, chosen.shape[0])
 
 
@@ -350,4 +355,4 @@ def preference_loss_and_grad(chosen: torch.Tensor, rejected: torch.Tensor, ref_c
     chosen, rejected = chosen.detach(), rejected.detach()
     keep, rest = _describe_preference(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, label_smoothing, kind, average)
     out, gc, gr = _preference_forward(_pack_preference(keep, rest), chosen, rejected, True, grad_scale)
-    return out[0], _preference_info(out, chosen.shape[0]), gc, gr
+    return _loss(out), _preference_info(out, chosen.shape[0]), gc, gr

@@ -481,6 +481,29 @@ def test_preference_gradient_against_differences():
             assert abs(d - float(x.grad.view(-1)[i])) <= step ** 2 + 8 * H * float(f(c).abs() + 1) / step
 
 
+@gpu
+def test_losses_may_be_changed_in_place():
+    """`loss /= n` and `loss += other` as gradient accumulation writes them, with and without a gradient; what `info` holds stays as it is."""
+    lp, old, ref, adv, m = (t.cuda() for t in _policy_case(6, 40, torch.float32, "random", "rows"))
+    for f in (lambda x: P.policy_loss(x, adv, old, ref, m, kl_coef=0.1), lambda x: P.preference_loss(x[:3], x[3:], ref[:3], ref[3:], m[:3], m[3:])):
+        x, y = lp.clone().requires_grad_(), lp.clone().requires_grad_()
+        loss, info = f(x)
+        kept = {k: t.clone() for k, t in info.items()}
+        value = loss.detach().clone()
+        loss /= 4
+        loss += 1
+        loss.backward()
+        other, _ = f(y)
+        (other / 4 + 1).backward()
+        assert torch.equal(loss.detach(), value / 4 + 1) and torch.equal(x.grad, y.grad)
+        assert all(torch.equal(info[k], kept[k]) and not info[k].requires_grad for k in info)
+        z = torch.ones((), device="cuda", requires_grad=True)
+        loss, info = f(lp)
+        loss += z
+        loss.backward()
+        assert float(z.grad) == 1.0 and not any(t.requires_grad for t in info.values())
+
+
 # -- streams, graphs, two calls at once ------------------------------------------------------------------------------------------------------
 @gpu
 def test_losses_on_another_stream_and_in_a_graph():
