@@ -17,6 +17,7 @@ and `rejected` -- are differentiated: everything else is a constant of the graph
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from sde_sampler_amd import _lib as L
@@ -33,6 +34,11 @@ def _code(name: str, t: torch.Tensor, device=None) -> int:
     if code is None:
         raise L.SdehUnsupported(-2, f"{name}: {t.dtype} (the kernels take float32, bfloat16 and float16)")
     return code
+
+
+def _no_tangent(name: str, t: torch.Tensor) -> None:
+    if unpack_dual(t).tangent is not None:  # (the kernels see its values only; a result without a tangent would pass for a constant)
+        raise NotImplementedError(f"{name}: forward-mode differentiation is not implemented")
 
 
 def _constant(t: torch.Tensor | None) -> torch.Tensor | None:
@@ -88,6 +94,7 @@ def step_log_ratio(control: torch.Tensor, behaviour: torch.Tensor | None, increm
     if control.ndim != 3 or control.shape[2] < 1:
         raise ValueError(f"step_log_ratio: control must be [steps, batch, dim], got {tuple(control.shape)}")
     code = _code("step_log_ratio", control)
+    _no_tangent("step_log_ratio", control)
     for name, t in (("behaviour", behaviour), ("increments", increments)):
         if t is None and name == "behaviour":
             continue
@@ -115,6 +122,7 @@ def _describe_policy(log_prob, advantage, old, ref, mask, clip_low, clip_high, d
         raise ValueError(f"policy_loss: log_prob must be [rows, steps], got {tuple(log_prob.shape)}")
     dev, shape = log_prob.device, log_prob.shape
     code = _code("policy_loss", log_prob)
+    _no_tangent("policy_loss", log_prob)
     for name, t in (("old_log_prob", old), ("ref_log_prob", ref)):
         if t is not None and (t.shape != shape or t.dtype != log_prob.dtype or t.device != dev):
             raise ValueError(f"policy_loss: {name} is {tuple(t.shape)} {t.dtype} on {t.device}, log_prob {tuple(shape)} {log_prob.dtype} on {dev}")
@@ -246,6 +254,7 @@ def _describe_preference(chosen, rejected, ref_chosen, ref_rejected, chosen_mask
     code = _code("preference_loss", chosen)
     tensors = []
     for name, x, ref, mask in (("chosen", chosen, ref_chosen, chosen_mask), ("rejected", rejected, ref_rejected, rejected_mask)):
+        _no_tangent("preference_loss", x)
         if x.dtype != chosen.dtype or x.device != chosen.device:
             raise ValueError(f"preference_loss: chosen is {chosen.dtype} on {chosen.device}, rejected {x.dtype} on {x.device}")
         if ref is not None and (ref.shape != x.shape or ref.dtype != x.dtype or ref.device != x.device):

@@ -10,6 +10,7 @@ from pathlib import Path
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from sde_sampler_amd import _lib as L
 from sde_sampler_amd.losses import policy as P
@@ -640,6 +641,23 @@ def test_gradients_are_differentiable_once():
         assert torch.equal(first, again)
         with pytest.raises(RuntimeError):  # (a gradient of the gradient: there is none, and none is made up)
             again.sum().backward()
+
+
+@gpu
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent would be lost without a word."""
+    lp = torch.zeros(3, 4, device="cuda")
+    u = torch.zeros(3, 4, 2, device="cuda")
+    ones = torch.ones(3, device="cuda")
+    with fwad.dual_level():
+        x, w = fwad.make_dual(lp, torch.ones_like(lp)), fwad.make_dual(u, torch.ones_like(u))
+        for f in (lambda: P.policy_loss(x, ones), lambda: P.preference_loss(x, lp), lambda: P.preference_loss(lp, x),
+                  lambda: P.step_log_ratio(w, None, u, ones), lambda: P.policy_loss(x.t(), torch.ones(4, device="cuda"))):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(NotImplementedError, match="forward"):
+                    f()
+        P.policy_loss(lp, ones)
+        P.step_log_ratio(u, None, u, ones)
 
 
 @gpu
