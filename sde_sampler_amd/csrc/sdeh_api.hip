@@ -1993,7 +1993,7 @@ static int32_t step_log_ratio(const char* who, const void* control, const void* 
     return fail(SDEH_ERR_INVALID, "%s: null pointer", who);
   if (n_steps > INT64_MAX / 16 / batch / dim) return fail(SDEH_ERR_INVALID, "%s: too many elements", who);
   const int rc = launch_step_log_ratio(control, behaviour, increments, dt, grad, n_steps, batch, dim, dtype, out, (hipStream_t)stream);
-  return rc == SDEH_OK ? SDEH_OK : fail(rc, rc == SDEH_ERR_UNSUPPORTED ? "%s: more rows than one launch holds" : "%s: launch failed", who);
+  return rc == SDEH_OK ? SDEH_OK : fail(rc, "%s: launch failed", who);
 }
 
 int32_t sdeh_step_log_ratio(const void* control, const void* behaviour, const void* increments, const float* dt, int64_t n_steps, int64_t batch,

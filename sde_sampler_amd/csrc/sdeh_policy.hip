@@ -9,6 +9,15 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// A launch holds fewer than 2^32 threads: kernels that take one piece of work a workgroup take theirs in several launches where there are more, each told
+// how many workgroups the launches before it had.
+constexpr long long kMostBlocks = 0xFFFFFFFFll / kThreads;
+
+template <typename F>
+void launch_pieces(long long blocks, const F& launch) {
+  for (long long first = 0; first < blocks; first += kMostBlocks) launch(first, dim3((unsigned)(blocks - first < kMostBlocks ? blocks - first : kMostBlocks)));
+}
+
 // i = row * steps + col; by 32-bit arithmetic where i fits it (a 64-bit division takes a hundred instructions and more)
 __device__ __forceinline__ void split_index(long long i, long long steps, long long& row, long long& col) {
   if ((unsigned long long)i >> 32 == 0ull && (unsigned long long)steps >> 32 == 0ull) {
@@ -42,6 +51,7 @@ struct RatioArgs {
   void* out;
   long long rows_total, batch;
   int dim, rows, group;  // rows per stretch, lanes per row
+  long long first;       // workgroups of the launches before
 };
 
 template <typename T, int V, bool BACK>
@@ -49,7 +59,7 @@ __global__ __launch_bounds__(kThreads) void ratio_kernel(RatioArgs a) {
   __shared__ float term[BACK ? 1 : kStretch + kStretch / 32];
   __shared__ float row_dt[kStretchRows];
   __shared__ float row_g[BACK ? kStretchRows : 1];
-  const long long r0 = (long long)blockIdx.x * a.rows;
+  const long long r0 = (a.first + blockIdx.x) * a.rows;
   const int nr = (int)(a.rows_total - r0 < a.rows ? a.rows_total - r0 : a.rows);
   const int d = a.dim, n = nr * d;
   const long long t0 = r0 / a.batch;  // (uniform over the workgroup)
@@ -130,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void ratio_forward_kernel(RatioArgs a, un
   constexpr int kTurns = 2, kVectors = kTurns * kThreads;  // (four turns of fp32 took 140 registers: 60 instead of 54 us for 200 x 2048 x 50)
   __shared__ float before[kVectors], after[kVectors];
   __shared__ float row_dt[kStretchRows + 1];
-  const long long r0 = (long long)blockIdx.x * a.rows;
+  const long long r0 = (a.first + blockIdx.x) * a.rows;
   const int nr = (int)(a.rows_total - r0 < a.rows ? a.rows_total - r0 : a.rows);
   const int d = a.dim, n = nr * d, whole = n / V;
   const T* u = static_cast<const T*>(a.u) + r0 * d;
@@ -200,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void ratio_forward_kernel(RatioArgs a, un
 // rows longer than kStagedDim: a workgroup sums one
 template <typename T>
 __global__ __launch_bounds__(kThreads) void ratio_long_kernel(RatioArgs a) {
-  const long long row = blockIdx.x, base = row * a.dim;
+  const long long row = a.first + blockIdx.x, base = row * a.dim;
   const T* u = static_cast<const T*>(a.u) + base;
   const T* v = a.v == nullptr ? nullptr : static_cast<const T*>(a.v) + base;
   const T* dw = static_cast<const T*>(a.dw) + base;
@@ -216,7 +226,7 @@ __global__ __launch_bounds__(kThreads) void ratio_long_kernel(RatioArgs a) {
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void ratio_long_back_kernel(RatioArgs a) {
-  const long long row = blockIdx.x, base = row * a.dim;
+  const long long row = a.first + blockIdx.x, base = row * a.dim;
   const T* u = static_cast<const T*>(a.u) + base;
   const T* v = a.v == nullptr ? nullptr : static_cast<const T*>(a.v) + base;
   const T* dw = static_cast<const T*>(a.dw) + base;
@@ -231,11 +241,13 @@ __global__ __launch_bounds__(kThreads) void ratio_long_back_kernel(RatioArgs a) 
 template <typename T, bool BACK>
 int launch_ratio_t(RatioArgs a, hipStream_t stream) {
   if (a.dim > kStagedDim) {
-    if (a.rows_total > 0x7FFFFFFFll) return SDEH_ERR_UNSUPPORTED;
-    if (BACK)
-      hipLaunchKernelGGL(ratio_long_back_kernel<T>, dim3((unsigned)a.rows_total), dim3(kThreads), 0, stream, a);
-    else
-      hipLaunchKernelGGL(ratio_long_kernel<T>, dim3((unsigned)a.rows_total), dim3(kThreads), 0, stream, a);
+    launch_pieces(a.rows_total, [&](long long first, dim3 grid) {
+      a.first = first;
+      if (BACK)
+        hipLaunchKernelGGL(ratio_long_back_kernel<T>, grid, dim3(kThreads), 0, stream, a);
+      else
+        hipLaunchKernelGGL(ratio_long_kernel<T>, grid, dim3(kThreads), 0, stream, a);
+    });
     return hipGetLastError() == hipSuccess ? SDEH_OK : SDEH_ERR_HIP;
   }
   // whole rows, a multiple of eight of them: every stretch then starts at a multiple of 16 bytes
@@ -243,21 +255,23 @@ int launch_ratio_t(RatioArgs a, hipStream_t stream) {
   a.rows = rows > kStretchRows ? kStretchRows : rows;
   a.group = 1;
   while (a.group < 64 && a.group * 2 * a.rows <= kThreads && a.group * 2 <= a.dim) a.group *= 2;
-  const long long blocks = (a.rows_total + a.rows - 1) / a.rows;
-  if (blocks > 0x7FFFFFFFll) return SDEH_ERR_UNSUPPORTED;
   constexpr int V = 16 / (int)sizeof(T);
   const bool wide = aligned_to(a.u, 16) && aligned_to(a.dw, 16) && (a.v == nullptr || aligned_to(a.v, 16)) && (!BACK || aligned_to(a.out, 16));
-  if (wide && !BACK && a.dim >= V) {
+  const bool split = wide && !BACK && a.dim >= V;
+  if (split) {
     a.rows = 2 * kThreads * V / a.dim / V * V;  // (whole rows, V of them: at least V as dim <= 512)
     a.group = 1;                                // (for the vectors of a row, not its elements)
     while (a.group < 64 && a.group * 2 * a.rows <= kThreads && a.group * 2 * V <= a.dim) a.group *= 2;
-    const long long stretches = (a.rows_total + a.rows - 1) / a.rows;
-    if (stretches > 0x7FFFFFFFll) return SDEH_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((ratio_forward_kernel<T, V>), dim3((unsigned)stretches), dim3(kThreads), 0, stream, a, (unsigned)((0x100000000ull + a.dim - 1) / a.dim));
-  } else if (wide)
-    hipLaunchKernelGGL((ratio_kernel<T, V, BACK>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((ratio_kernel<T, 1, BACK>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+  }
+  launch_pieces((a.rows_total + a.rows - 1) / a.rows, [&](long long first, dim3 grid) {
+    a.first = first;
+    if (split)
+      hipLaunchKernelGGL((ratio_forward_kernel<T, V>), grid, dim3(kThreads), 0, stream, a, (unsigned)((0x100000000ull + a.dim - 1) / a.dim));
+    else if (wide)
+      hipLaunchKernelGGL((ratio_kernel<T, V, BACK>), grid, dim3(kThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL((ratio_kernel<T, 1, BACK>), grid, dim3(kThreads), 0, stream, a);
+  });
   return hipGetLastError() == hipSuccess ? SDEH_OK : SDEH_ERR_HIP;
 }
 
@@ -265,7 +279,7 @@ int launch_ratio_t(RatioArgs a, hipStream_t stream) {
 
 int launch_step_log_ratio(const void* u, const void* v, const void* dw, const float* dt, const float* g, long long n_steps, long long batch,
                           int dim, int dtype, void* out, hipStream_t stream) {
-  RatioArgs a{u, v, dw, dt, g, out, n_steps * batch, batch, dim, 0, 0};
+  RatioArgs a{u, v, dw, dt, g, out, n_steps * batch, batch, dim, 0, 0, 0};
   if (g != nullptr)
     return dtype == SDEH_F32 ? launch_ratio_t<float, true>(a, stream)
                              : dtype == SDEH_BF16 ? launch_ratio_t<bf16_t, true>(a, stream) : launch_ratio_t<f16_t, true>(a, stream);
@@ -838,6 +852,7 @@ constexpr int kPairBlocks = 256;
 struct PreferenceArgs {
   SdehPreferenceLoss p;
   int splits;               // parts of a row
+  long long first;          // workgroups of the launches before (preference_sum_kernel)
   long long chunk;          // entries of a part
   double* sum;              // [2 pairs][splits]   scratch
   long long* count;         // [2 pairs][splits]
@@ -916,8 +931,8 @@ __device__ __forceinline__ void row_share(const SdehPreferenceSide& s, long long
 // one workgroup a part of a row
 template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void preference_sum_kernel(PreferenceArgs a) {
-  const long long line = blockIdx.x / a.splits;
-  const int split = blockIdx.x % a.splits;
+  const long long part = a.first + blockIdx.x, line = part / a.splits;
+  const int split = (int)(part - line * a.splits);
   const bool second = line >= a.p.pairs;
   const SdehPreferenceSide& s = second ? a.p.rejected : a.p.chosen;
   const long long lo = split * a.chunk, hi = lo + a.chunk < s.steps ? lo + a.chunk : s.steps;
@@ -927,8 +942,8 @@ __global__ __launch_bounds__(kThreads) void preference_sum_kernel(PreferenceArgs
   sum = block_sum<kThreads>(sum);
   count = block_sum<kThreads>(count);
   if (threadIdx.x == 0) {
-    a.sum[blockIdx.x] = sum;
-    a.count[blockIdx.x] = count;
+    a.sum[part] = sum;
+    a.count[part] = count;
   }
 }
 
@@ -1205,12 +1220,13 @@ int launch_preference_t(PreferenceArgs a, hipStream_t stream) {
     else
       hipLaunchKernelGGL((preference_short_kernel<T, 1>), grid, dim3(kThreads), 0, stream, a);
   } else {
-    const long long blocks = 2 * p.pairs * a.splits;
-    if (blocks > 0x7FFFFFFFll) return SDEH_ERR_UNSUPPORTED;
-    if (wide)
-      hipLaunchKernelGGL((preference_sum_kernel<T, V>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
-    else
-      hipLaunchKernelGGL((preference_sum_kernel<T, 1>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+    launch_pieces(2 * p.pairs * a.splits, [&](long long first, dim3 grid) {
+      a.first = first;
+      if (wide)
+        hipLaunchKernelGGL((preference_sum_kernel<T, V>), grid, dim3(kThreads), 0, stream, a);
+      else
+        hipLaunchKernelGGL((preference_sum_kernel<T, 1>), grid, dim3(kThreads), 0, stream, a);
+    });
   }
   const long long per = a.splits == 1 ? kThreads : kThreads / 64;
   long long pair_blocks = (p.pairs + per - 1) / per;

@@ -754,3 +754,44 @@ def test_step_log_ratio_past_32_bit_offsets():
     y = y.detach()
     assert float(y[-1, -1]) == 7 * (2.0 * 0.5 - 0.25 * 4.0) and float(y[-1, -2]) == 0.25 and int((y != 0).sum()) == 1
     assert bool((u.grad[-1, -1] == -0.5).all()) and float(u.grad[-1, -2, 0]) == 0.0 and int((u.grad != 0.5).sum()) == 8
+
+
+MANY = (1 << 24) + 99  # workgroups of 256 threads: more than a launch holds
+
+
+@gpu
+def test_step_log_ratio_of_more_rows_than_a_launch_holds():
+    """A workgroup a row (dim > 512): forward and backward, the rows around the first launch's end and the last ones."""
+    _room(80)
+    T, d = 7, 513
+    B = -(-MANY // T)
+    u = torch.zeros(T, B, d, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    dw = torch.full((T, B, d), 0.5, device="cuda", dtype=torch.bfloat16)
+    dt = torch.arange(1, T + 1, device="cuda") * 0.125
+    rows = [0, (1 << 24) - 2, (1 << 24) - 1, 1 << 24, T * B - 1]
+    with torch.no_grad():
+        u.view(-1, d)[rows, 512] = 1.0
+    y = P.step_log_ratio(u, None, dw, dt)
+    y.backward(torch.ones_like(y))
+    y = y.detach().view(-1)
+    assert y[rows].cpu().tolist() == [0.5 - 0.5 * 0.125 * (r // B + 1) for r in rows] and int((y != 0).sum()) == len(rows)
+    g = u.grad.view(-1, d)
+    assert g[rows, 512].cpu().tolist() == [0.5 - 0.125 * (r // B + 1) for r in rows]
+    assert int((g != 0.5).sum()) == len(rows)
+
+
+@gpu
+def test_preference_loss_of_more_rows_than_a_launch_holds():
+    _room(64)
+    pairs = MANY // 2 + 1  # two rows of a pair, a workgroup each
+    x = torch.zeros(pairs, 1025, device="cuda", dtype=torch.bfloat16)
+    y = torch.zeros(pairs, 1, device="cuda", dtype=torch.bfloat16)
+    x[0, 0], x[-1, -1], y[-1, 0], y[-50, 0] = 2.0, 3.0, 1.0, 4.0
+    loss, info, gx, gy = P.preference_loss_and_grad(x, y, beta=1.0, kind="hinge", grad_scale=float(pairs))
+    c, r = info["chosen_rewards"], info["rejected_rewards"]
+    assert float(c[0]) == 2.0 and float(c[-1]) == 3.0 and int((c != 0).sum()) == 2
+    assert float(r[-1]) == 1.0 and float(r[-50]) == 4.0 and int((r != 0).sum()) == 2
+    # losses: 0 for the first and the last pair, 5 for the 50th from the end, 1 for every other; slopes -1 where the loss is not 0
+    assert abs(float(loss) * pairs - (pairs - 3 + 5)) <= 2 * H * pairs
+    flat = gx.sum(1, dtype=torch.float32)
+    assert float(flat[0]) == float(flat[-1]) == 0.0 and int((flat != -1025).sum()) == 2 and int((gy != 1).sum()) == 2
