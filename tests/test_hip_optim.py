@@ -720,6 +720,51 @@ def test_policy_steps_on_stored_trajectories():
     assert torch.isfinite(loss) and info["chosen_rewards"].shape == (B // 2,) and float(opt.grad_norm) > 0.0
 
 
+@gpu
+@pytest.mark.parametrize("name", ["cfg1_dw_dis_lv", "gmm50_pis_headline"])
+def test_documented_steps_on_stored_trajectories(name):
+    """The documentation's example: the control called along the paths is the one that drove them, and its gradients are those of the formulas."""
+    prob = problems.build(problems.baseline_spec(name), device="cuda:0")  # (its own grid: in 20 steps some paths of the double well reach |x| = 4000, where
+    torch.manual_seed(3)                                                  # the k3 term of a moved control overflows in the formula itself)
+    x0 = prob.prior.sample((128,))
+
+    def control(xs):
+        return torch.stack([prob.ctrl(t, x) for t, x in zip(prob.ts, xs)])
+
+    opt = AdamW(prob.ctrl.parameters(), lr=1e-3, weight_decay=0.0, max_grad_norm=1.0)
+    dt = prob.ts.diff()
+    noise = torch.randn(dt.numel(), *x0.shape, device="cuda")
+    res = prob.eval(x0, compute_weights=True, return_traj=True, noise=noise)
+    dw = noise * dt.sqrt()[:, None, None]
+    weight = res.weights.squeeze(-1)
+    advantage = (weight - weight.mean()) / weight.std()
+    with torch.no_grad():
+        v = control(res.xs[:-1])
+        # x + (drift + diff u) dt + diff dW; three layers of 64 products in fp32 are right to 1e-4 of their size, 1e-3 is asked for
+        for k, (t, x) in enumerate(zip(prob.ts, res.xs[:-1])):
+            diff = prob.sde.diff(t, x)
+            want = x + (prob.sde.drift(t, x) + diff * v[k]) * dt[k] + diff * dw[k]
+            tol = 1e-3 * diff * dt[k] * (1 + v[k].abs()) + 16 * H * (x.abs() + want.abs() + 1)
+            assert ((res.xs[k + 1] - want).abs() <= tol).all()
+    params = [p for p in prob.ctrl.parameters() if p.requires_grad]
+    for k in range(3):
+        u = control(res.xs[:-1])
+        ratio = P.step_log_ratio(u, v, dw, dt).t()
+        assert k or not ratio.any()
+        loss, info = P.policy_loss(ratio, advantage, ref_log_prob=torch.zeros_like(ratio), kl_coef=0.05)
+        opt.zero_grad()
+        loss.backward()
+        e = control(res.xs[:-1]) - v
+        r = (e * dw - 0.5 * dt[:, None, None] * e * e).sum(-1).t()
+        want = torch.maximum(-advantage[:, None] * r.exp(), -advantage[:, None] * r.exp().clamp(0.8, 1.2)) + 0.05 * (torch.exp(-r) - 1 + r)
+        for p, g in zip(params, torch.autograd.grad(want.mean(), params, allow_unused=True)):
+            assert (p.grad is None) == (g is None)
+            if g is not None:  # (both sides sum 12 800 rows' contributions in fp32, in different orders)
+                assert (p.grad - g).abs().max() <= 2e-5 * g.abs().max() + 1e-7
+        opt.step()
+        assert torch.isfinite(loss) and float(info["n_valid"]) == ratio.numel()
+
+
 # -- refusals ----------------------------------------------------------------------------------------------------------------------------------
 def test_constructor_refuses():
     p = [torch.nn.Parameter(torch.zeros(3))]
