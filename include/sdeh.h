@@ -548,7 +548,7 @@ typedef enum { SDEH_F32 = 0, SDEH_BF16 = 1, SDEH_F16 = 2 } SdehDtype;
 /* Log-ratio of the Gaussian Euler-Maruyama steps of two controls of one SDE (the Girsanov weight of a single step; the quantity that
  * losses/oc.py:204-219 accumulates over a trajectory), for paths driven by `increments` dW under the control `behaviour` v:
  *   log_ratio[t, b] = sum_d (u - v) dW  -  1/2 dt[t] sum_d (u - v)^2
- * control, behaviour (NULL = 0), increments: [n_steps, batch, dim] contiguous, one dtype;  dt [n_steps] fp32;  log_ratio [n_steps, batch] fp32.
+ * control, behaviour (NULL = 0), increments: [n_steps, batch, dim] contiguous, one dtype, dim at most 2^30;  dt [n_steps] fp32;  log_ratio [n_steps, batch] fp32.
  * _backward: grad_control = grad[t, b] (dW - dt (u - v)), grad [n_steps, batch] fp32, grad_control like control. */
 int32_t sdeh_step_log_ratio(const void* control, const void* behaviour, const void* increments, const float* dt, int64_t n_steps,
                             int64_t batch, int32_t dim, int32_t dtype, float* log_ratio, void* stream);

@@ -33,6 +33,7 @@ KL_ESTIMATORS = {"k1": 1, "k2": 2, "k3": 3}
 REDUCTIONS = {"steps": 0, "rows": 1, "sum": 2}
 PREFERENCE_KINDS = {"logistic": 0, "hinge": 1, "square": 2}
 MOMENT_BLOCK = 256
+MAX_DIM = 1 << 30  # of step_log_ratio
 # structs of the loss / optimizer entry points, packed in one go (native alignment, as in include/sdeh.h)
 POLICY_LOSS = struct.Struct("@" + "Pqq" * 5 + "qq4i4d")
 PREFERENCE_LOSS = struct.Struct("@" + ("Pqq" * 3 + "q") * 2 + "q3i2d")

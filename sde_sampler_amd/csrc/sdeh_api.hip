@@ -1987,7 +1987,7 @@ static bool dtype_ok(int32_t t) { return t == SDEH_F32 || t == SDEH_BF16 || t ==
 
 static int32_t step_log_ratio(const char* who, const void* control, const void* behaviour, const void* increments, const float* dt, const float* grad,
                               int64_t n_steps, int64_t batch, int32_t dim, int32_t dtype, void* out, bool back, void* stream) {
-  if (n_steps < 0 || batch < 0 || dim < 1 || !dtype_ok(dtype)) return fail(SDEH_ERR_INVALID, "%s: bad size or type", who);
+  if (n_steps < 0 || batch < 0 || dim < 1 || dim > 1 << 30 || !dtype_ok(dtype)) return fail(SDEH_ERR_INVALID, "%s: bad size or type", who);
   if (n_steps == 0 || batch == 0) return SDEH_OK;
   if (control == nullptr || increments == nullptr || dt == nullptr || out == nullptr || (back && grad == nullptr))
     return fail(SDEH_ERR_INVALID, "%s: null pointer", who);

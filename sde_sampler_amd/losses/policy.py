@@ -91,8 +91,8 @@ def step_log_ratio(control: torch.Tensor, behaviour: torch.Tensor | None, increm
     increments  [T, B, d]  the Brownian increments sqrt(dt) * noise that were added under `behaviour`
     dt          [T]        step sizes
     `control`, `behaviour` and `increments` have one type; tensors that are not contiguous are copied."""
-    if control.ndim != 3 or control.shape[2] < 1:
-        raise ValueError(f"step_log_ratio: control must be [steps, batch, dim], got {tuple(control.shape)}")
+    if control.ndim != 3 or not 1 <= control.shape[2] <= L.MAX_DIM:
+        raise ValueError(f"step_log_ratio: control must be [steps, batch, dim] with 1 <= dim <= 2^30, got {tuple(control.shape)}")
     code = _code("step_log_ratio", control)
     _no_tangent("step_log_ratio", control)
     for name, t in (("behaviour", behaviour), ("increments", increments)):

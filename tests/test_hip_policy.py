@@ -570,6 +570,18 @@ def test_cpu_tensors_are_refused():
         P.preference_loss(x, x)
 
 
+@pytest.mark.parametrize("d", [(1 << 30) + 1, (1 << 31) - 1, 1 << 31, (1 << 32) + 7])
+def test_step_log_ratio_refuses_dims_past_what_it_indexes(d):
+    """Cut to 32 bits a dim of 2^32 + 7 would be 7, and an index of 32 bits that goes on in steps of 256 passes 2^31 behind a row of 2^31 - 1."""
+    u = torch.zeros(1).expand(1, 1, d)
+    with pytest.raises(ValueError, match="dim"):
+        P.step_log_ratio(u, None, u, torch.ones(1))
+    if d < 1 << 31:
+        lib = L.load()
+        assert lib.sdeh_step_log_ratio(64, None, 64, 64, 0, 2, d, 0, 64, None) == lib.sdeh_step_log_ratio(64, None, 64, 64, 1, 1, d, 0, 64, None) == -1
+        assert lib.sdeh_step_log_ratio_backward(64, None, 64, 64, 64, 1, 1, d, 0, 64, None) == -1
+
+
 def test_c_entries_refuse_bad_arguments():
     lib = L.load()
     ok = lambda **k: L.POLICY_LOSS.pack(*(64, 4, 1) * 5, k.get("rows", 2), k.get("steps", 4), k.get("dtype", 0), 0, k.get("kl", 3), k.get("red", 0),  # noqa: E731
