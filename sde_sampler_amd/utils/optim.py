@@ -33,6 +33,8 @@ class _Bucket:
         self.flat = {"step": zeros(len(params), torch.float32), "exp_avg": zeros(n, kind), "exp_avg_sq": zeros(n, kind)}
         if bits == 8:
             self.flat.update(exp_avg_top=zeros(self.blocks, torch.uint8), exp_avg_sq_top=zeros(self.blocks, torch.uint8))
+        # what a step writes and has a version (inference tensors have none)
+        self.versioned = [[t for t in ts if not t.is_inference()] for ts in (params, self.flat.values())]
         self.states = []
         self.table = np.zeros((len(params), L.ADAMW_TENSOR_WORDS), dtype=np.int64)
         for i, (p, size, b) in enumerate(zip(params, self.sizes, blocks)):
@@ -68,9 +70,10 @@ class _Bucket:
             grad.append(g.data_ptr())
         self.table[:, 0] = param
         self.table[:, 1] = grad
+        written, flats = self.versioned
         if not missing:
-            return self.table, keep, [*self.params, *self.flat.values()]
-        return self.table[self.table[:, 0] != 0], keep, [*(p for p in self.params if p.grad is not None), *self.flat.values()]
+            return self.table, keep, written + flats
+        return self.table[self.table[:, 0] != 0], keep, [p for p in written if p.grad is not None] + flats
 
 
 class AdamW(torch.optim.Optimizer):
@@ -314,11 +317,11 @@ class AdamW(torch.optim.Optimizer):
         head = L.ADAMW.pack(self.max_grad_norm or 0.0, 0 if ok is None else ok.data_ptr(), 0 if norm is None else norm.data_ptr(),
                             self.seed & 0xFFFFFFFF, len(groups))
         L.call("sdeh_adamw_step", self._device, head, b"".join(groups), table.ctypes.data, self._scratch.data_ptr())
-        if norm is not None:
+        if norm is not None and not norm.is_inference():
             written.append(norm)
         # (written behind torch's back: whoever saved one of them for a backward pass, or cached what it held, is told here -- also where `ok` is False,
         # which the host does not know)
-        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+        torch.autograd.graph.increment_version(written)
         return loss
 
     _hooked_step = torch.optim.Optimizer.profile_hook_step(_step)

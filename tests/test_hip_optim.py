@@ -384,6 +384,24 @@ def test_a_step_is_seen_by_autograd(bits):
     assert p._version > version and opt.grad_norm._version > norm
 
 
+@gpu
+def test_steps_in_inference_mode():
+    """Tensors made there have no version to move; a parameter without a gradient keeps its version, so that graphs that saved it go backward."""
+    p, frozen = _params([12, 12], torch.float32)
+    frozen.requires_grad_(False)
+    opt = AdamW([p, frozen], max_grad_norm=1.0, lr=0.5, weight_decay=0.0)
+    p.grad = torch.ones_like(p)
+    x = torch.ones(12, device="cuda", requires_grad=True)
+    loss = (frozen * x).sum()
+    start = p.detach().clone()
+    with torch.inference_mode():
+        opt.step()
+    opt.step()
+    loss.backward()
+    assert torch.equal(x.grad, frozen) and float(opt.state[p]["step"]) == 2.0
+    assert ((start - p.detach()) - 1.0).abs().max() <= 2.0 ** -20  # (two steps of lr along a gradient that does not change, roundings of values below 2)
+
+
 # -- state dicts ------------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
