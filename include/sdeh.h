@@ -579,7 +579,7 @@ typedef struct {
   double clip_low, clip_high, dual_clip /* 0 = none */, kl_coef;
 } SdehPolicyLoss;
 int64_t sdeh_policy_loss_scratch_floats(int64_t rows, int64_t steps, int32_t masked); /* 0: none is used (scratch still is not NULL) */
-/* out (nullable) [5] fp32 = loss, sum w surrogate, sum w kl, clipped share of the valid entries, their number.
+/* out (nullable) [5] fp32 = loss, sum w surrogate, sum w kl, clipped share of the valid entries, their number (rounded above 2^24).
  * grad (nullable) [rows, steps] contiguous, dtype: d loss / d log_prob x grad_factor x *grad_scale (fp32 on the device, NULL = 1).
  * reuse_counts != 0: scratch still holds what an earlier call with a mask of the same values and strides, and the same reduction, left there (a loss's backward pass). */
 int32_t sdeh_policy_loss(const SdehPolicyLoss* p, float* scratch, int32_t reuse_counts, const float* grad_scale, float grad_factor, float* out,

@@ -10,9 +10,11 @@ several steps when the losses account for the control having moved since: with `
 (`Problem.eval(..., noise=)` gives the paths, `noise * dt.sqrt()` the increments; the reference accumulates the same increments of the log-ratio
 in losses/oc.py:204-219.)  `policy_loss` and `preference_loss` take any log-probabilities [rows, steps], so they serve sequence models as well.
 
-All functions run on the HIP device, on torch's current stream, never synchronise and may be captured into a graph.  fp32, bf16 and fp16; sums
-are held in 64 bits, results in fp32, gradients in the type of what they belong to.  Only the first argument(s) -- `control`, `log_prob`, `chosen`
-and `rejected` -- are differentiated: everything else is a constant of the graph.
+All functions run on the HIP device, on torch's current stream, never synchronise and may be captured into a graph (a captured backward pass wants
+fresh leaves, as any: utils/graphs.py; the `*_and_grad` forms have no autograd graph).  fp32, bf16 and fp16; a log-ratio's sum over the coordinates is
+held in 32 bits, the losses' sums over rows and steps in 64 (the policy loss adds the 4 or 8 entries of a 16-byte vector in 32 bits first); results are
+fp32, gradients of the type of what they belong to.  Only the first argument(s) -- `control`, `log_prob`, `chosen` and `rejected` -- are differentiated, in
+reverse mode and once: everything else is a constant of the graph.
 """
 from __future__ import annotations
 
@@ -216,7 +218,8 @@ def policy_loss(log_prob: torch.Tensor, advantage: torch.Tensor, old_log_prob: t
     ref_log_prob  like log_prob; None: no KL term
     mask          bool (or uint8), broadcastable to [rows, steps]; entries it leaves out do not count, whatever they hold
     reduction     "steps": mean over the valid entries; "rows": mean over the rows that have any, of their means; "sum"
-    info          0-d fp32 tensors: policy and kl (the two terms, reduced like the loss), clip_fraction, n_valid
+    info          0-d fp32 tensors: policy and kl (the two terms, reduced like the loss), clip_fraction, n_valid (exact up to 2^24 entries, rounded
+                  beyond; the weights and shares come from the exact number)
     Without a valid entry the loss and its gradient are 0.  A log-probability of -inf in a valid entry gives what the formula gives."""
     tensors, rest = _describe_policy(log_prob, advantage, old_log_prob, ref_log_prob, mask, clip_low, clip_high, dual_clip, kl_coef, kl, reduction)
     x, adv, old, ref, mask = tensors

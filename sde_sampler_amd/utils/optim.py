@@ -206,7 +206,8 @@ class AdamW(torch.optim.Optimizer):
         return out
 
     def load_state_dict(self, state_dict):
-        """Values are copied into this optimizer's own buffers, learning rates on the device into their own tensors: a captured step keeps working on them.
+        """Values are copied into this optimizer's own buffers, learning rates on the device into their own tensors: a captured step keeps working on them
+        (numbers -- a float lr, betas, the seed -- are part of the capture and stay what they were).
         A state dict of torch.optim.AdamW (or Adam, without weight decay) fits 32-bit moments; its flags about how to compute are dropped, those about what
         (amsgrad, maximize) are refused.  A state dict that is refused leaves everything as it was."""
         loaded, held = {}, {}
